@@ -155,6 +155,99 @@ typedef struct p0k_attn_args {
   float scale, cap;
 } p0k_attn_args;
 
+/* ---- key / value cache in 8 bits, and rotary positions (no counterpart in the reference) ----------------------------
+ * Rows of Q / K / V have 128 f16 values a head. A tensor of H heads is (buf, off in bytes, size, rs, hs): row r of head h
+ * starts rs * r + hs * h halves behind off (0: rs = 128, hs = rows * rs, the `heads` epilogue's layout; token-major:
+ * rs = H * 128, hs = 128). Offsets 16-byte aligned, strides multiples of 8.
+ *
+ * p0k_batch: the rows of a call belong to B sequences, rows cu[b] .. cu[b + 1] - 1 to sequence b (int32, not decreasing,
+ * B + 1 of them); row r is that sequence's token t = pos[b] + r - cu[b] (int32). Rows outside [cu[0], cu[B]) are left as
+ * they are. slot[b] (int32, optional: b) says which sequence of the cache it is. All three are read on the device, so a
+ * captured graph serves other lengths when their contents change. A sequence with pos < 0 or a slot outside the cache has
+ * no tokens. No slot may come twice in one p0k_kv_append. At most 2^24 rows and 2^20 sequences a call. */
+typedef struct p0k_batch {
+  const int32_t *pos_buf; uint64_t pos_off, pos_size;     /* offsets and sizes in bytes */
+  const int32_t *cu_buf; uint64_t cu_off, cu_size;
+  const int32_t *slot_buf; uint64_t slot_off, slot_size;
+  uint32_t B, rows;                                       /* rows: of the tensors (cu is held to it) */
+} p0k_batch;
+
+/* p0k_kv_cache: keys and values of `slots` sequences, in blocks of 64 tokens. A whole block lies in a page of the pool:
+ * int8 codes of each kv head's 64 x 128 keys and values with one fp32 scale each (value = code * scale). Block k of
+ * sequence s is page table[s][k] (int32). The block that a sequence is still filling and the one before it are held in
+ * f16 in its tail. Buffers: p0k_kv_code_bytes / p0k_kv_scale_bytes / p0k_kv_tail_bytes; their inner layout is the
+ * library's. Pages of whole blocks may be shared by sequences. A table entry outside [0, pages): the block is not there
+ * (not written, not seen, read back as zeros); it may stay unset until the block before it is whole. */
+typedef struct p0k_kv_cache {
+  void *code_buf; uint64_t code_off, code_size;           /* codes, tail: 16-byte aligned; scales: 8-byte */
+  float *scale_buf; uint64_t scale_off, scale_size;
+  void *tail_buf; uint64_t tail_off, tail_size;
+  const int32_t *table_buf; uint64_t table_off, table_size;   /* [slots][max_pages] */
+  uint32_t pages, slots, max_pages, Hkv;
+} p0k_kv_cache;
+
+/* rotary positions: y = x rotated by the angles a_i = t f_i of its token t, i < rd / 2: pairs (2 i, 2 i + 1) or, mode
+ * P0K_ROPE_HALF, (i, i + rd / 2) become mscale * (x1 cos a - x2 sin a, x2 cos a + x1 sin a); values from rd on are copied.
+ * f_i = theta^(-2 i / rd), or freqs[i] where freqs (rd / 2 doubles in host memory, read by the call) is given; then
+ *   P0K_ROPE_LINEAR  f_i / factor
+ *   P0K_ROPE_BANDS   f_i (u + (1 - u) / factor), u = clamp((orig f_i / 2 pi - low) / (high - low), 0, 1): pairs that turn
+ *                    more than `high` times within orig tokens keep their frequency, those below `low` are stretched
+ * Angles are computed in 64-bit fractions of a turn: exact to fp32 at any position. rd 0 = 128, theta 0 = 10000, mscale 0
+ * = 1. y may be x itself (same offset and strides; no other overlap). Positions may be negative here. batch.cu_buf NULL:
+ * pos is one position per row (B and slot are not used). */
+enum { P0K_ROPE_PLAIN = 0, P0K_ROPE_LINEAR = 1, P0K_ROPE_BANDS = 2 };
+typedef struct p0k_rope_args {
+  uint32_t struct_size;
+  const void *x_buf; uint64_t x_off, x_size, x_rs, x_hs;
+  void *y_buf; uint64_t y_off, y_size, y_rs, y_hs;
+  p0k_batch batch;
+  uint32_t H, rd;
+  int32_t mode, scaling;                                  /* P0K_ROPE_INTERLEAVED | HALF; P0K_ROPE_PLAIN | LINEAR | BANDS */
+  double theta, factor, orig, low, high;
+  const double *freqs;
+  float mscale;
+} p0k_rope_args;
+
+/* kv_append: rows of K and V [Hkv] into the cache as tokens pos[b] .. of sequence b. Values are held to +-65504, NaN counts
+ * as 0. A block that becomes whole is quantised from the f16 values of all of its tokens: scale = max |x| / 127 in fp32 (1
+ * where all are 0), code = x / scale rounded to the nearest, ties to even. So the cache depends on the tokens only, not on
+ * how many came with a call. A sequence may go back: pos may be any place from the start of the block before the one that
+ * was being filled (64 tokens back or more; rejected draft tokens). Tokens from max_pages * 64 on are not kept. */
+typedef struct p0k_kv_append_args {
+  uint32_t struct_size;
+  p0k_kv_cache cache;
+  p0k_batch batch;
+  const void *k_buf; uint64_t k_off, k_size, k_rs, k_hs;
+  const void *v_buf; uint64_t v_off, v_size, v_rs, v_hs;
+} p0k_kv_append_args;
+
+/* kv_read: row r of K and V = the cached token pos[b] + r - cu[b] of sequence b, in f16 (code * scale rounded once; the
+ * open block's values as they are), zeros where there is none. len[b] (int32 [B]): tokens that sequence b holds. */
+typedef struct p0k_kv_read_args {
+  uint32_t struct_size;
+  p0k_kv_cache cache;
+  p0k_batch batch;
+  const int32_t *len_buf; uint64_t len_off, len_size;
+  void *k_buf; uint64_t k_off, k_size, k_rs, k_hs;
+  void *v_buf; uint64_t v_off, v_size, v_rs, v_hs;
+} p0k_kv_read_args;
+
+/* kv_attention: O [rows][ldo] f16, head h at column h * 128 = softmax(scale q.k) v over the cached tokens j that the query
+ * at token t sees: j <= t and, with a window, j > t - window or j < sinks. The cache holds the batch's own rows already
+ * (p0k_kv_append comes first): sequence b has pos[b] + cu[b + 1] - cu[b] tokens. Query head h reads kv head h / (Hq / Hkv).
+ * A row that sees nothing is 0. Zero fields: ldo = Hq * 128, scale = 1 / sqrt(128), window: none, cap: none (cap * tanh(s /
+ * cap) otherwise). o: 8-byte aligned, ldo a multiple of 4. Pages wholly outside every row's window are not read. The keys
+ * are divided over workgroups through a fixed workspace of the context (not in a capture begun by the caller). */
+typedef struct p0k_kv_attn_args {
+  uint32_t struct_size;
+  p0k_kv_cache cache;
+  p0k_batch batch;
+  const void *q_buf; uint64_t q_off, q_size, q_rs, q_hs;
+  void *o_buf; uint64_t o_off, o_size; uint32_t ldo;
+  uint32_t Hq, window, sinks;
+  float scale, cap;
+} p0k_kv_attn_args;
+
 typedef struct p0k_tile { uint32_t bm, bn; int32_t kernel; } /* kernel: 0 = MFMA GEMM (register-staged), 1 = GEMV (q4, M <= 4), 2 = MFMA GEMV (M <= 16), 3 = MFMA GEMM (load-to-LDS),
    4 = short-call GEMV (q4, q8 or f16, M <= 4, 16-row items) */
   p0k_tile;
@@ -235,6 +328,19 @@ int p0k_rowstats(p0k_ctx *ctx, const p0k_rowstats_args *a);
 int p0k_attention_check(const p0k_attn_args *a);
 int p0k_attention(p0k_ctx *ctx, const p0k_attn_args *a);
 double p0k_attention_flops(const p0k_attn_args *a);
+
+/* rotary positions and the 8-bit key / value cache. The *_check functions validate only (no context, no GPU) */
+int p0k_rope_check(const p0k_rope_args *a);
+int p0k_rope(p0k_ctx *ctx, const p0k_rope_args *a);
+uint64_t p0k_kv_code_bytes(uint32_t pages, uint32_t Hkv);
+uint64_t p0k_kv_scale_bytes(uint32_t pages, uint32_t Hkv);
+uint64_t p0k_kv_tail_bytes(uint32_t slots, uint32_t Hkv);
+int p0k_kv_append_check(const p0k_kv_append_args *a);
+int p0k_kv_append(p0k_ctx *ctx, const p0k_kv_append_args *a);
+int p0k_kv_read_check(const p0k_kv_read_args *a);
+int p0k_kv_read(p0k_ctx *ctx, const p0k_kv_read_args *a);
+int p0k_kv_attention_check(const p0k_kv_attn_args *a);
+int p0k_kv_attention(p0k_ctx *ctx, const p0k_kv_attn_args *a);
 
 /* pixstats(gpu, a)               src/ops/video.js:317  */
 int p0k_pixstats(p0k_ctx *ctx, const p0k_pixstats_args *a);

@@ -39,6 +39,12 @@ int prepare_rowstats(const p0k_rowstats_args *a, std::string *err);
 int prepare_pixstats(const p0k_pixstats_args *a, std::string *err);
 struct AttnParams;
 int prepare_attention(const p0k_attn_args *a, AttnParams *out, std::string *err);
+struct RopeParams;
+struct KvParams;
+int prepare_rope(const p0k_rope_args *a, RopeParams *out, std::string *err);
+int prepare_kv_append(const p0k_kv_append_args *a, KvParams *out, std::string *err);
+int prepare_kv_read(const p0k_kv_read_args *a, KvParams *out, std::string *err);
+int prepare_kv_attention(const p0k_kv_attn_args *a, KvParams *out, std::string *err);
 // what: 1 = partial rows, 2 = finalize, 3 = both
 int prepare_gn(const p0k_gn_args *a, int what, std::string *err);
 }  // namespace p0k

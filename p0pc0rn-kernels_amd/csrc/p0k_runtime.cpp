@@ -16,6 +16,7 @@
 #include "../../include/p0k.h"
 #include "p0k_device.h"
 #include "p0k_internal.h"
+#include "p0k_kv.h"
 #include "p0k_launch.h"
 
 namespace {
@@ -888,6 +889,106 @@ int p0k_attention(p0k_ctx *c, const p0k_attn_args *a) {
   if (runs > 1) c->capture_ws = true;
   hipError_t e = p0k::launch_attention(p, (int)tune.cus, tune.attn_bq, runs, c->ws_attn, c->ws_attn_cnt, c->stream);
   if (e != hipSuccess) return hip_err(e, "attention launch");
+  return P0K_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ key / value cache
+static int check_live_batch(p0k_ctx *c, const p0k_batch &b, const char *op) {
+  if (int r = check_live(c, b.pos_buf, b.pos_size, op, "pos")) return r;
+  if (b.cu_buf)
+    if (int r = check_live(c, b.cu_buf, b.cu_size, op, "cu")) return r;
+  return b.slot_buf ? check_live(c, b.slot_buf, b.slot_size, op, "slot") : P0K_OK;
+}
+static int check_live_cache(p0k_ctx *c, const p0k_kv_cache &k, const char *op) {
+  int r;
+  if ((r = check_live(c, k.code_buf, k.code_size, op, "code")) || (r = check_live(c, k.scale_buf, k.scale_size, op, "scale")) ||
+      (r = check_live(c, k.tail_buf, k.tail_size, op, "tail")) || (r = check_live(c, k.table_buf, k.table_size, op, "table")))
+    return r;
+  return P0K_OK;
+}
+
+int p0k_rope_check(const p0k_rope_args *a) {
+  std::string err;
+  const int r = p0k::prepare_rope(a, nullptr, &err);
+  return r ? set_err(r, err) : P0K_OK;
+}
+int p0k_rope(p0k_ctx *c, const p0k_rope_args *a) {
+  if (!c) return set_err(P0K_E_ARG, "rope: NULL context");
+  std::string err;
+  p0k::RopeParams p;
+  int r = p0k::prepare_rope(a, &p, &err);
+  if (r) return set_err(r, err);
+  if ((r = check_live(c, a->x_buf, a->x_size, "rope", "x")) || (r = check_live(c, a->y_buf, a->y_size, "rope", "y")) ||
+      (r = check_live_batch(c, a->batch, "rope")))
+    return r;
+  HIPCHK(hipSetDevice(c->device), "hipSetDevice");
+  std::lock_guard<std::mutex> order(c->enq);
+  hipError_t e = p0k::launch_rope(p, c->stream);
+  if (e != hipSuccess) return hip_err(e, "rope launch");
+  return P0K_OK;
+}
+
+int p0k_kv_append_check(const p0k_kv_append_args *a) {
+  std::string err;
+  const int r = p0k::prepare_kv_append(a, nullptr, &err);
+  return r ? set_err(r, err) : P0K_OK;
+}
+int p0k_kv_append(p0k_ctx *c, const p0k_kv_append_args *a) {
+  if (!c) return set_err(P0K_E_ARG, "kv_append: NULL context");
+  std::string err;
+  p0k::KvParams p;
+  int r = p0k::prepare_kv_append(a, &p, &err);
+  if (r) return set_err(r, err);
+  if ((r = check_live_cache(c, a->cache, "kv_append")) || (r = check_live_batch(c, a->batch, "kv_append")) ||
+      (r = check_live(c, a->k_buf, a->k_size, "kv_append", "k")) || (r = check_live(c, a->v_buf, a->v_size, "kv_append", "v")))
+    return r;
+  HIPCHK(hipSetDevice(c->device), "hipSetDevice");
+  std::lock_guard<std::mutex> order(c->enq);
+  hipError_t e = p0k::launch_kv_append(p, c->stream);
+  if (e != hipSuccess) return hip_err(e, "kv_append launch");
+  return P0K_OK;
+}
+
+int p0k_kv_read_check(const p0k_kv_read_args *a) {
+  std::string err;
+  const int r = p0k::prepare_kv_read(a, nullptr, &err);
+  return r ? set_err(r, err) : P0K_OK;
+}
+int p0k_kv_read(p0k_ctx *c, const p0k_kv_read_args *a) {
+  if (!c) return set_err(P0K_E_ARG, "kv_read: NULL context");
+  std::string err;
+  p0k::KvParams p;
+  int r = p0k::prepare_kv_read(a, &p, &err);
+  if (r) return set_err(r, err);
+  if ((r = check_live_cache(c, a->cache, "kv_read")) || (r = check_live_batch(c, a->batch, "kv_read")) ||
+      (r = check_live(c, a->len_buf, a->len_size, "kv_read", "len")) || (r = check_live(c, a->k_buf, a->k_size, "kv_read", "k")) ||
+      (r = check_live(c, a->v_buf, a->v_size, "kv_read", "v")))
+    return r;
+  HIPCHK(hipSetDevice(c->device), "hipSetDevice");
+  std::lock_guard<std::mutex> order(c->enq);
+  hipError_t e = p0k::launch_kv_read(p, c->stream);
+  if (e != hipSuccess) return hip_err(e, "kv_read launch");
+  return P0K_OK;
+}
+
+int p0k_kv_attention_check(const p0k_kv_attn_args *a) {
+  std::string err;
+  const int r = p0k::prepare_kv_attention(a, nullptr, &err);
+  return r ? set_err(r, err) : P0K_OK;
+}
+int p0k_kv_attention(p0k_ctx *c, const p0k_kv_attn_args *a) {
+  if (!c) return set_err(P0K_E_ARG, "kv_attention: NULL context");
+  std::string err;
+  p0k::KvParams p;
+  int r = p0k::prepare_kv_attention(a, &p, &err);
+  if (r) return set_err(r, err);
+  if ((r = check_live_cache(c, a->cache, "kv_attention")) || (r = check_live_batch(c, a->batch, "kv_attention")) ||
+      (r = check_live(c, a->q_buf, a->q_size, "kv_attention", "q")) || (r = check_live(c, a->o_buf, a->o_size, "kv_attention", "o")))
+    return r;
+  HIPCHK(hipSetDevice(c->device), "hipSetDevice");
+  std::lock_guard<std::mutex> order(c->enq);
+  hipError_t e = p0k::launch_kv_attention(p, c->stream);
+  if (e != hipSuccess) return hip_err(e, "kv_attention launch");
   return P0K_OK;
 }
 

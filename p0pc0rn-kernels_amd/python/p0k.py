@@ -113,6 +113,135 @@ def attn_args(a, resolve):
     return s
 
 
+def _operand(name, *more):
+    return [(name + "_buf", C.c_void_p), (name + "_off", C.c_uint64), (name + "_size", C.c_uint64)] + [(name + m, t) for m, t in more]
+
+
+_STRIDES = (("_rs", C.c_uint64), ("_hs", C.c_uint64))
+
+
+class Batch(C.Structure):
+    _fields_ = _operand("pos") + _operand("cu") + _operand("slot") + [("B", C.c_uint32), ("rows", C.c_uint32)]
+
+
+class KvCache(C.Structure):
+    _fields_ = (_operand("code") + _operand("scale") + _operand("tail") + _operand("table") +
+                [(n, C.c_uint32) for n in ("pages", "slots", "max_pages", "Hkv")])
+
+
+class RopeArgs(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32)] + _operand("x", *_STRIDES) + _operand("y", *_STRIDES) + [("batch", Batch)] +
+                [(n, C.c_uint32) for n in ("H", "rd")] + [(n, C.c_int32) for n in ("mode", "scaling")] +
+                [(n, C.c_double) for n in ("theta", "factor", "orig", "low", "high")] +
+                [("freqs", C.POINTER(C.c_double)), ("mscale", C.c_float)])
+
+
+class KvAppendArgs(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32), ("cache", KvCache), ("batch", Batch)] + _operand("k", *_STRIDES) +
+                _operand("v", *_STRIDES))
+
+
+class KvReadArgs(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32), ("cache", KvCache), ("batch", Batch)] + _operand("len") +
+                _operand("k", *_STRIDES) + _operand("v", *_STRIDES))
+
+
+class KvAttnArgs(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32), ("cache", KvCache), ("batch", Batch)] + _operand("q", *_STRIDES) +
+                _operand("o") + [(n, C.c_uint32) for n in ("ldo", "Hq", "window", "sinks")] +
+                [("scale", C.c_float), ("cap", C.c_float)])
+
+
+ROPE_MODE = {"interleaved": 0, "half": 1}
+ROPE_SCALING = {"plain": 0, "linear": 1, "bands": 2}
+
+
+def _set_operand(s, name, a, resolve, strides=False):
+    """{buf, off, rs, hs} (or the buffer itself) into the struct's fields"""
+    if not isinstance(a, dict):
+        a = {"buf": a}
+    p, n = resolve(a["buf"])
+    setattr(s, name + "_buf", p)
+    setattr(s, name + "_off", _get(a, "off", 0))
+    setattr(s, name + "_size", n)
+    if strides:
+        setattr(s, name + "_rs", _get(a, "rs", 0))
+        setattr(s, name + "_hs", _get(a, "hs", 0))
+
+
+def _set_batch(s, b, resolve):
+    for n in ("pos", "cu", "slot"):
+        if b.get(n) is not None:
+            _set_operand(s, n, b[n], resolve)
+    s.B, s.rows = _get(b, "B", 0), b["rows"]
+
+
+def _set_cache(s, c, resolve):
+    for n in ("code", "scale", "tail", "table"):
+        _set_operand(s, n, c[n], resolve)
+    s.pages, s.slots, s.max_pages, s.Hkv = c["pages"], c["slots"], c["max_pages"], c["Hkv"]
+
+
+def rope_args(a, resolve):
+    """{x, y: {buf, off, rs, hs}, H, batch: {pos, cu, B, rows}, rd, mode: 'interleaved' | 'half', theta, scaling: {kind:
+    'linear' | 'bands', factor, orig, low, high}, freqs: rd / 2 numbers, mscale} -> RopeArgs (p0k_rope of p0k.h). Without y
+    the rotation is in place."""
+    s = RopeArgs()
+    s.struct_size = C.sizeof(RopeArgs)
+    _set_operand(s, "x", a["x"], resolve, True)
+    _set_operand(s, "y", a.get("y") or a["x"], resolve, True)
+    _set_batch(s.batch, a["batch"], resolve)
+    s.H, s.rd, s.mode = a["H"], _get(a, "rd", 0), ROPE_MODE[a.get("mode") or "interleaved"]
+    s.theta, s.mscale = _get(a, "theta", 0.0), _get(a, "mscale", 0.0)
+    sc = a.get("scaling")
+    if sc:
+        s.scaling = ROPE_SCALING[sc["kind"]]
+        s.factor, s.orig, s.low, s.high = (_get(sc, n, 0.0) for n in ("factor", "orig", "low", "high"))
+    if a.get("freqs") is not None:
+        if len(a["freqs"]) != (s.rd or 128) // 2:
+            raise ValueError(f"rope: {len(a['freqs'])} frequencies for rd {s.rd or 128}")
+        s.freqs = (C.c_double * len(a["freqs"]))(*a["freqs"])    # (the struct keeps the array)
+    return s
+
+
+def kv_append_args(a, resolve):
+    """{cache, batch: {pos, cu, slot, B, rows}, k, v: {buf, off, rs, hs}} -> KvAppendArgs (p0k_kv_append of p0k.h)"""
+    s = KvAppendArgs()
+    s.struct_size = C.sizeof(KvAppendArgs)
+    _set_cache(s.cache, a["cache"], resolve)
+    _set_batch(s.batch, a["batch"], resolve)
+    _set_operand(s, "k", a["k"], resolve, True)
+    _set_operand(s, "v", a["v"], resolve, True)
+    return s
+
+
+def kv_read_args(a, resolve):
+    """{cache, batch, len, k, v: {buf, off, rs, hs}} -> KvReadArgs (p0k_kv_read of p0k.h)"""
+    s = KvReadArgs()
+    s.struct_size = C.sizeof(KvReadArgs)
+    _set_cache(s.cache, a["cache"], resolve)
+    _set_batch(s.batch, a["batch"], resolve)
+    _set_operand(s, "len", a["len"], resolve)
+    _set_operand(s, "k", a["k"], resolve, True)
+    _set_operand(s, "v", a["v"], resolve, True)
+    return s
+
+
+def kv_attention_args(a, resolve):
+    """{cache, batch, q: {buf, off, rs, hs}, o: {buf, off, ld}, Hq, window, sinks, scale, cap} -> KvAttnArgs (p0k_kv_attention
+    of p0k.h)"""
+    s = KvAttnArgs()
+    s.struct_size = C.sizeof(KvAttnArgs)
+    _set_cache(s.cache, a["cache"], resolve)
+    _set_batch(s.batch, a["batch"], resolve)
+    _set_operand(s, "q", a["q"], resolve, True)
+    _set_operand(s, "o", a["o"], resolve)
+    s.ldo = _get(a["o"], "ld", 0) if isinstance(a["o"], dict) else 0
+    s.Hq, s.window, s.sinks = a["Hq"], _get(a, "window", 0), _get(a, "sinks", 0)
+    s.scale, s.cap = _get(a, "scale", 0.0), _get(a, "cap", 0.0)
+    return s
+
+
 class Tile(C.Structure):
     _fields_ = [("bm", C.c_uint32), ("bn", C.c_uint32), ("kernel", C.c_int32)]
 
@@ -135,6 +264,8 @@ EXPORTS = [
     "p0k_free", "p0k_drain_pool", "p0k_pool_stats_get", "p0k_upload", "p0k_download", "p0k_copy", "p0k_sync",
     "p0k_gemm_check", "p0k_gemm", "p0k_gemm_flops", "p0k_select_tile", "p0k_rowstats_check", "p0k_rowstats",
     "p0k_attention_check", "p0k_attention", "p0k_attention_flops",
+    "p0k_rope_check", "p0k_rope", "p0k_kv_code_bytes", "p0k_kv_scale_bytes", "p0k_kv_tail_bytes",
+    "p0k_kv_append_check", "p0k_kv_append", "p0k_kv_read_check", "p0k_kv_read", "p0k_kv_attention_check", "p0k_kv_attention",
     "p0k_pixstats", "p0k_gn_part_bytes", "p0k_gn_partial", "p0k_gn_finalize", "p0k_groupnorm_stats",
     "p0k_event_create", "p0k_event_record", "p0k_event_elapsed_ms", "p0k_event_destroy",
     "p0k_tensor_bytes", "p0k_pack_q4", "p0k_pack_q8", "p0k_pack_f16",
@@ -172,6 +303,12 @@ def lib():
             "p0k_pixstats": ([P, C.POINTER(PixstatsArgs)], I), "p0k_gn_part_bytes": ([C.c_uint32], U64),
             "p0k_attention_check": ([C.POINTER(AttnArgs)], I), "p0k_attention": ([P, C.POINTER(AttnArgs)], I),
             "p0k_attention_flops": ([C.POINTER(AttnArgs)], C.c_double),
+            "p0k_rope_check": ([C.POINTER(RopeArgs)], I), "p0k_rope": ([P, C.POINTER(RopeArgs)], I),
+            "p0k_kv_code_bytes": ([C.c_uint32, C.c_uint32], U64), "p0k_kv_scale_bytes": ([C.c_uint32, C.c_uint32], U64),
+            "p0k_kv_tail_bytes": ([C.c_uint32, C.c_uint32], U64),
+            "p0k_kv_append_check": ([C.POINTER(KvAppendArgs)], I), "p0k_kv_append": ([P, C.POINTER(KvAppendArgs)], I),
+            "p0k_kv_read_check": ([C.POINTER(KvReadArgs)], I), "p0k_kv_read": ([P, C.POINTER(KvReadArgs)], I),
+            "p0k_kv_attention_check": ([C.POINTER(KvAttnArgs)], I), "p0k_kv_attention": ([P, C.POINTER(KvAttnArgs)], I),
             "p0k_gn_partial": ([P, C.POINTER(GnArgs), C.POINTER(C.c_uint32)], I),
             "p0k_gn_finalize": ([P, C.POINTER(GnArgs)], I), "p0k_groupnorm_stats": ([P, C.POINTER(GnArgs)], I),
             "p0k_event_create": ([P, C.POINTER(P)], I), "p0k_event_record": ([P, P], I),
@@ -414,6 +551,54 @@ class Device:
         self._sync_env()
         _chk(lib().p0k_attention(self.ctx, C.byref(s)))
         return lib().p0k_attention_flops(C.byref(s))
+
+    def rope_raw(self, s):
+        _chk(lib().p0k_rope(self.ctx, C.byref(s)))
+
+    def rope(self, a):
+        """rotary positions on the rows of a batch (rope_args has the fields)"""
+        self.rope_raw(rope_args(a, self.resolve))
+
+    def kv_cache(self, Hkv, pages, slots, max_pages, table=None):
+        """The buffers of an 8-bit key / value cache (p0k_kv_cache of p0k.h) as the `cache` of the kv_* calls: `pages` pages of
+        64 tokens for all kv heads, `slots` sequences of up to max_pages blocks. table: int32 [slots][max_pages] page
+        numbers, -1 where there is none; without one, sequence s owns pages s * max_pages on."""
+        L, own = lib(), table is None
+        if own:
+            t = np.full((slots, max_pages), -1, np.int32)
+            n = min(pages, slots * max_pages)
+            t.reshape(-1)[:n] = np.arange(n)
+            table = self.upload(t)
+        return {"code": self.buffer(L.p0k_kv_code_bytes(pages, Hkv)), "scale": self.buffer(L.p0k_kv_scale_bytes(pages, Hkv)),
+                "tail": self.buffer(L.p0k_kv_tail_bytes(slots, Hkv)), "table": table,
+                "pages": pages, "slots": slots, "max_pages": max_pages, "Hkv": Hkv, "own_table": own}
+
+    def kv_cache_free(self, cache):
+        """gives the cache's buffers back (a table that came from the caller stays the caller's)"""
+        for n in ("code", "scale", "tail") + (("table",) if cache["own_table"] else ()):
+            self.free(cache[n])
+
+    def kv_append_raw(self, s):
+        _chk(lib().p0k_kv_append(self.ctx, C.byref(s)))
+
+    def kv_append(self, a):
+        """rows of K / V into the cache (kv_append_args has the fields)"""
+        self.kv_append_raw(kv_append_args(a, self.resolve))
+
+    def kv_read_raw(self, s):
+        _chk(lib().p0k_kv_read(self.ctx, C.byref(s)))
+
+    def kv_read(self, a):
+        """cached rows back as f16 (kv_read_args has the fields)"""
+        self.kv_read_raw(kv_read_args(a, self.resolve))
+
+    def kv_attention_raw(self, s):
+        self._sync_env()
+        _chk(lib().p0k_kv_attention(self.ctx, C.byref(s)))
+
+    def kv_attention(self, a):
+        """attention over the cache (kv_attention_args has the fields)"""
+        self.kv_attention_raw(kv_attention_args(a, self.resolve))
 
     def pixstats(self, x, V, Cc, r, eps=0.0, ro=0, x_off=0):
         """pixstats(gpu, {x, r, V, C, eps, ro}) of src/ops/video.js:317."""
