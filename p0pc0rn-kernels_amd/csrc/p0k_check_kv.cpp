@@ -143,6 +143,9 @@ int prepare_kv_attention(const p0k_kv_attn_args *a, KvParams *out, std::string *
   NEED(a->o_off % 8 == 0 && o.ldo % 4 == 0 && o.ldo >= a->Hq * 128,
        "kv_attention: o offset 8-byte aligned, ldo a multiple of 4 covering Hq * 128");
   if (o.rows) CHECK(fits(err, "kv_attention", "o", a->o_off, ((uint64_t)(o.rows - 1) * o.ldo + a->Hq * 128) * 2, a->o_size));
+  // the kernels count (unit of 32 tokens, head, 16 rows) in 32 bits
+  NEED((unsigned __int128)a->cache.max_pages * 2 * o.Hkv * ((uint64_t)o.rows * (a->Hq / o.Hkv) / 16 + o.B) < (1ull << 32),
+       "kv_attention: max_pages %u with %u rows of %u heads is too large for one call", a->cache.max_pages, o.rows, a->Hq);
   o.K = (const uint16_t *)((const uint8_t *)a->q_buf + a->q_off);
   o.Ko = (uint16_t *)((uint8_t *)a->o_buf + a->o_off);
   o.Hq = a->Hq; o.window = a->window; o.sinks = a->sinks;

@@ -1,8 +1,10 @@
 // p0k_kv.h — the 8-bit key / value cache: its layout, the kernels' parameters and the host-side launchers.
 //
 // A block is 64 tokens of one sequence. A page of the pool holds a block of every kv head: for each head 8 KB of key codes
-// and 8 KB of value codes, and one fp32 scale each. Codes lie in the order in which the attention kernels' matrix
-// instructions take them, so that a wave loads its operands from memory straight into registers, 1 KB an instruction:
+// and 8 KB of value codes, and one fp32 scale each. A code's byte is code + 128 (1 to 255): bytes 0x64 b are the f16 number
+// 1024 + b, so two codes become f16 with one byte permutation and one packed subtraction. Codes lie in the order in which
+// the attention kernels' matrix instructions take them, so that a wave loads its operands from memory straight into
+// registers, 1 KB an instruction:
 //   keys    16-byte pieces of 16 consecutive d of one token:   [half of 32 tokens][16-token tile][64 d][16 d][token % 16]
 //   values  16-byte pieces of 8 tokens of d and of d + 16:     [half of 32 tokens][32 d][token group][d % 16]
 // where token group q of a half holds its tokens 4 q .. 4 q + 3 and 16 + 4 q .. + 3: the eight tokens of which a lane of the
@@ -12,6 +14,8 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include "p0k_device.h"
 
 namespace p0k {
 
@@ -110,11 +114,29 @@ __device__ __forceinline__ uint32_t kv_page(const KvParams &p, uint32_t slot, ui
   const int32_t v = p.table[(uint64_t)slot * p.max_pages + block];
   return v >= 0 && (uint32_t)v < p.pages ? (uint32_t)v : 0xffffffffu;
 }
+// the four codes of a word as f16 (exact)
+__device__ __forceinline__ void kv_f16(uint32_t w, f16x2 *lo, f16x2 *hi) {
+  const f16x2 k1152 = {(f16)1152.0f, (f16)1152.0f};
+  *lo = as_h2(perm(0x64646464u, w, 0x04010400u)) - k1152;
+  *hi = as_h2(perm(0x64646464u, w, 0x04030402u)) - k1152;
+}
+__device__ __forceinline__ f16x8 kv_f16x8(uint32_t a, uint32_t b) {
+  f16x2 v[4];
+  kv_f16(a, &v[0], &v[1]);
+  kv_f16(b, &v[2], &v[3]);
+  return (f16x8){v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
+}
 #endif
+
+// attention over runs of keys: its workspace (partial results of a workgroup's first and last group, and a counter each)
+constexpr uint32_t kva_part(uint32_t rows) { return rows * (KV_D + 2); }          // floats of one partial result
+uint64_t kv_attention_part_bytes(int cus);
+unsigned kv_attention_counters(int cus);
 
 hipError_t launch_rope(const RopeParams &p, hipStream_t s);
 hipError_t launch_kv_append(const KvParams &p, hipStream_t s);
 hipError_t launch_kv_read(const KvParams &p, hipStream_t s);
-hipError_t launch_kv_attention(const KvParams &p, hipStream_t s);
+// ws: part / cnt may be used
+hipError_t launch_kv_attention(const KvParams &p, int cus, bool ws, float *part, unsigned *cnt, hipStream_t s);
 
 }  // namespace p0k

@@ -1,66 +1,472 @@
 // p0k_kvattn.hip — attention over the 8-bit key / value cache (layout: p0k_kv.h).
 //
 //   o_i = sum_j softmax_j(scale q_i.k_j) v_j over the cached tokens j that query i sees, k = code * its block's scale
-#include "p0k_device.h"
 #include "p0k_kv.h"
+#include "p0k_launch.h"
+
+#include <algorithm>
 
 namespace p0k {
 
-// One wave per query row and head: a lane owns a token of a 64-token block for the scores, two d for the sums.
-__global__ __launch_bounds__(64) void k_kv_attn_row(KvParams p) {
-  __shared__ float sq[KV_D];
-  const uint32_t r = blockIdx.x, hq = blockIdx.y, lane = threadIdx.x, h = hq / (p.Hq / p.Hkv);
-  uint32_t lo = 0, hi = p.B;
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) >> 1;
-    if (kv_row0(p.cu, mid, p.rows) <= r) lo = mid;
-    else hi = mid;
+typedef unsigned short u16;
+
+// What a sequence asks of the kernel: units of 32 tokens, those of the sinks [0, su) and then from unit `lo` on (0 units:
+// nothing to do; a sequence that sees nothing has one that is all masked, for its rows have to be written)
+struct KvWork { KvSeq s; uint32_t end, su, lo, units, blocks, io; };   // io: the first unit of the open block, by its place
+
+template <int RB>                                 // rows of a block (a row: one query of one head)
+__device__ __forceinline__ KvWork kv_work(const KvParams &p, uint32_t b) {
+  KvWork w;
+  w.s = kv_seq(p, b);
+  const uint32_t cap = p.max_pages * KV_T, U32 = 32;
+  w.end = w.s.ok ? (w.s.pos + w.s.n < cap ? w.s.pos + w.s.n : cap) : 0u;
+  const uint32_t all = (w.end + U32 - 1) / U32;
+  w.lo = 0;
+  w.su = 0;
+  if (p.window && w.s.pos >= p.window) {
+    const uint32_t lo = (w.s.pos + 1 - p.window) / U32, su = p.sinks / U32 + (p.sinks % U32 != 0u);
+    w.lo = lo < all ? lo : all;
+    w.su = su < w.lo ? su : w.lo;
   }
-  const KvSeq s = kv_seq(p, lo);
-  if (r < s.r0 || r >= s.r0 + s.n) return;
-  const uint32_t cap = p.max_pages * KV_T, end = s.ok ? (s.pos + s.n < cap ? s.pos + s.n : cap) : 0u, tq = s.pos + (r - s.r0);
-  sq[lane] = h_val(p.K[p.krs * r + p.khs * hq + lane]);
-  sq[lane + 64] = h_val(p.K[p.krs * r + p.khs * hq + lane + 64]);
-  __syncthreads();
-  float m = -1e30f, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-  for (uint32_t blk = 0; blk * KV_T < end && blk * KV_T <= tq; blk++) {
-    if (p.window && blk * KV_T >= p.sinks && (uint64_t)(blk + 1) * KV_T + p.window <= (uint64_t)tq + 1) continue;
-    const bool open = blk == end / KV_T;
-    const uint32_t page = open ? 0u : kv_page(p, s.slot, blk);
-    if (page == 0xffffffffu) continue;
-    const uint8_t *kc = p.codes + kv_code_at(p, page, h, 0), *vc = kc + KV_HEAD;
-    const uint16_t *kt = p.tail + kv_tail_at(p, s.slot, blk, h, 0), *vt = kt + KV_HEAD;
-    const float sk = open ? 1.0f : p.scales[kv_scale_at(p, page, h, 0)], sv = open ? 1.0f : p.scales[kv_scale_at(p, page, h, 1)];
-    const uint32_t j = blk * KV_T + lane;
-    const bool see = j < end && j <= tq && (!p.window || (uint64_t)j + p.window > tq || j < p.sinks);
-    float a = 0.0f;
-    for (uint32_t d = 0; d < KV_D; d++)
-      a += sq[d] * (open ? (see ? h_val(kt[kv_ktail(lane, d)]) : 0.0f) : (float)(int8_t)kc[kv_kcode(lane, d)]);
-    a *= sk * p.scale;
-    if (p.cap > 0.0f) a = p.cap * tanhf(a / p.cap);
-    a = see ? a : -1e30f;
-    float mx = a;
-    for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-    const float mn = fmaxf(m, mx), f = expf(m - mn), e = see ? expf(a - mn) : 0.0f;
-    m = mn;
-    l = l * f + e;
-    o0 *= f;
-    o1 *= f;
-    for (uint32_t t = 0; t < KV_T; t++) {
-      const float w = __shfl(e, t, 64);
-      if (w == 0.0f) continue;
-      o0 += w * sv * (open ? h_val(vt[kv_vtail(t, 2 * lane)]) : (float)(int8_t)vc[kv_vcode(t, 2 * lane)]);
-      o1 += w * sv * (open ? h_val(vt[kv_vtail(t, 2 * lane + 1)]) : (float)(int8_t)vc[kv_vcode(t, 2 * lane + 1)]);
-    }
-  }
-  for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o, 64);
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  *(uint32_t *)(p.Ko + (uint64_t)r * p.ldo + hq * KV_D + 2 * lane) = pack2(o0 * inv, o1 * inv);
+  w.units = w.su + (all - w.lo);
+  if (w.units == 0) w.units = 1;
+  const uint32_t uo = w.end ? w.end / KV_T * (KV_T / U32) : 0xffffffffu;
+  w.io = w.su > uo ? uo : w.lo >= uo ? w.su : uo - w.lo + w.su;
+  w.blocks = (w.s.n * (p.Hq / p.Hkv) + RB - 1) / RB;
+  if (w.s.n == 0) w.units = 0;
+  return w;
 }
 
-hipError_t launch_kv_attention(const KvParams &p, hipStream_t s) {
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {                       // inclusive prefix sums over the wave
+  const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+  for (uint32_t o = 1; o < 64; o <<= 1) {
+    const uint32_t u = __shfl_up(v, o, 64);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+__device__ __forceinline__ uint32_t rfl(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ float rlf(float v, uint32_t l) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), l)); }
+
+// The keys of all sequences and kv heads are one line of units of 32 tokens (sequence, head, row block, unit), of which every
+// workgroup takes an equal run and every wave an equal part: a ragged batch is spread evenly, whatever its lengths. A group (sequence,
+// head, row block) that lies within a wave's part is finished by that wave. One that several waves share meets in LDS: each
+// leaves the part that it began with there, the wave that began the group adds them up. One that several workgroups share
+// meets in the workspace: the last to arrive adds up all of them, in order, so that results do not depend on timing.
+//
+// A lane owns a query (of the 16 columns of a 16x16x32 product) as in S^T = K Q^T, O^T += V^T P: the scores that it holds are
+// the B operand of the second product, and the cache's layout makes 16-byte loads the A operands of both. Codes are exact
+// in f16; the scales stay in fp32: the keys' multiplies the scores, and O is held in units of the current block's value scale.
+template <int NB, int NW, bool CAP>
+__global__ __launch_bounds__(64 * NW, NB == 1 ? 4 : NB == 2 ? 2 : 1) void k_kv_attn_split(KvParams p, uint32_t ws, float *part, uint32_t *cnt) {
+  constexpr uint32_t RB = 16 * NB, PART = kva_part(RB);
+  __shared__ __attribute__((aligned(16))) float sO[NW][NB * 8 * 64 * 4];
+  __shared__ float sM[NW][NB * 64], sL[NW][NB * 64];
+  __shared__ uint32_t sJob[2][6];                                                 // groups whose last part this workgroup brought
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = rfl(tid >> 6), r16 = lane & 15, q4 = lane >> 4;
+  const uint32_t rep = p.Hq / p.Hkv;
+  if (tid < 2) sJob[tid][0] = 0;
+
+  // ---- all units, and this workgroup's and wave's share of them
+  uint32_t T = 0, tot0 = 0;
+  for (uint32_t b0 = 0; b0 < p.B; b0 += 64) {
+    uint32_t t = 0;
+    if (b0 + lane < p.B) {
+      const KvWork w = kv_work<RB>(p, b0 + lane);
+      t = w.units * w.blocks * p.Hkv;
+    }
+    if (b0 == 0) tot0 = t;
+    T += __builtin_amdgcn_readlane(wave_scan(t), 63);
+  }
+  // the sequence of unit u, and its first unit
+  auto find = [&](uint32_t u, uint32_t *base) {
+    uint32_t at = 0;
+    for (uint32_t b0 = 0; b0 < p.B; b0 += 64) {
+      uint32_t t = tot0;
+      if (b0) {
+        t = 0;
+        if (b0 + lane < p.B) {
+          const KvWork w = kv_work<RB>(p, b0 + lane);
+          t = w.units * w.blocks * p.Hkv;
+        }
+      }
+      const uint32_t sum = wave_scan(t);
+      const uint64_t m = __ballot(at + sum > u);
+      if (m) {
+        const uint32_t f = (uint32_t)__builtin_ctzll(m);
+        *base = at + __builtin_amdgcn_readlane(sum - t, f);
+        return b0 + f;
+      }
+      at += __builtin_amdgcn_readlane(sum, 63);
+    }
+    *base = T;
+    return p.B;
+  };
+  uint32_t nwg = gridDim.x;
+  nwg = T < nwg ? T : nwg;
+  // (row blocks that share their keys go to one XCD)
+  const uint32_t blk = blockIdx.x, k = NB > 1 && nwg == gridDim.x && (nwg & 7u) == 0u ? (blk & 7u) * (nwg >> 3) + (blk >> 3) : blk;
+  if (k >= nwg) return;
+  const uint32_t uq = T / nwg, ur = T - uq * nwg;
+  auto first = [&](uint32_t i) { return uq * i + (i < ur ? i : ur); };            // the first unit of workgroup i
+  auto owner = [&](uint32_t u) { return u < ur * (uq + 1) ? u / (uq + 1) : ur + (u - ur * (uq + 1)) / uq; };
+  uint32_t wa = first(k), we = first(k + 1);
+  if (!ws) {
+    // no workspace: whole groups (a workgroup's run begins where the group of its first unit does)
+    for (int i = 0; i < 2; i++) {
+      uint32_t u = i ? we : wa, base;
+      if (u < T) {
+        const uint32_t b = rfl(find(u, &base));
+        const KvWork w = kv_work<RB>(p, b);
+        u -= (u - base) % w.units;
+      }
+      (i ? we : wa) = rfl(u);
+    }
+    if (wa >= we) return;
+  }
+  const uint32_t per = (we - wa + NW - 1) / NW;
+  auto wfirst = [&](uint32_t i) { const uint32_t u = wa + i * per; return u < we ? u : we; };
+  const uint32_t a = wfirst(wave), e = wfirst(wave + 1);
+
+  f32x4 acc[NB][8];
+  float m[NB], l[NB];
+  auto clear = [&] {
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+      m[nb] = -1.0e30f;
+      l[nb] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < 8; d++) acc[nb][d] = (f32x4){};
+    }
+  };
+  // this block's rows: O / l to memory
+  auto put = [&](const KvWork &w, uint32_t hk, uint32_t rb) {
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+      const uint32_t row = rb * RB + nb * 16 + r16, qi = row / rep, h = hk * rep + (row - qi * rep);
+      if (qi >= w.s.n) continue;
+      const float inv = l[nb] > 0.0f ? 1.0f / l[nb] : 0.0f;
+      u16 *o = p.Ko + (uint64_t)(w.s.r0 + qi) * p.ldo + h * KV_D + 4 * q4;
+#pragma unroll
+      for (int d = 0; d < 8; d++)
+        *(u32x2 *)(o + 16 * d) = (u32x2){pack2(acc[nb][d].x * inv, acc[nb][d].y * inv), pack2(acc[nb][d].z * inv, acc[nb][d].w * inv)};
+    }
+  };
+  const srsrc pr = stream_rsrc((const uint8_t *)part);
+  // this block's rows into the workspace; the last workgroup of the group to arrive takes it on (sJob)
+  auto leave = [&](const KvWork &w, uint32_t b, uint32_t hk, uint32_t rb, uint32_t g0, uint32_t out) {
+    const uint32_t base = (2 * k + out) * PART;
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+      const uint32_t row = rb * RB + nb * 16 + r16, at = base + (nb * 16 + r16) * KV_D + 4 * q4;
+      if (row / rep >= w.s.n) continue;
+#pragma unroll
+      for (int d = 0; d < 8; d++) sys_store128(pr, (at + 16 * d) * 4u, __builtin_bit_cast(u32x4, acc[nb][d]));
+      if (q4 == 0)
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, (f32x2){m[nb], l[nb]}), pr,
+                                              (int)((base + RB * KV_D + 2 * (nb * 16 + r16)) * 4u), 0, SC0_SC1);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    const uint32_t kf = owner(g0), kl = owner(g0 + w.units - 1);
+    uint32_t old = 0;
+    if (lane == 0) old = __hip_atomic_fetch_add(cnt + kf, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    if (rfl(old) == kl - kf && lane == 0) {
+      sJob[out][0] = 1; sJob[out][1] = kf; sJob[out][2] = kl; sJob[out][3] = b; sJob[out][4] = hk; sJob[out][5] = rb;
+    }
+  };
+
+  uint32_t u = a, base = 0, b = 0, hk = 0, rb = 0, g0 = 0;
+  KvWork w;
+  bool tail = false;                                                              // the registers hold a group that goes on
+  if (a < e) b = rfl(find(a, &base));
+  while (u < e) {
+    w = kv_work<RB>(p, b);
+    const uint32_t per_seq = w.units * w.blocks * p.Hkv;
+    if (u >= base + per_seq) {                                                    // (sequences without rows have no units)
+      base += per_seq;
+      b++;
+      continue;
+    }
+    const uint32_t gi = rfl((u - base) / w.units);
+    hk = rfl(gi / w.blocks);
+    rb = gi - hk * w.blocks;
+    g0 = base + gi * w.units;
+    const uint32_t i0 = u - g0, i1 = (e < g0 + w.units ? e : g0 + w.units) - g0;  // units of the group, by their place in it
+
+    // ---- the rows' queries: lane r16 holds row nb * 16 + r16, k step s = (64 d, 8 d) its d 64 (s / 2) + 16 q4 + 8 (s % 2) ..
+    f16x8 qf[NB][4];
+    uint32_t kmax[NB], wlo[NB];                                                   // the tokens that the row sees: below kmax, from wlo on or sinks
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+      uint32_t row = rb * RB + nb * 16 + r16;
+      const uint32_t last = w.s.n * rep - 1;
+      row = row < last ? row : last;
+      const uint32_t qi = row / rep, h = hk * rep + (row - qi * rep), t = w.s.pos + qi;
+      const u16 *q = p.K + p.krs * (w.s.r0 + qi) + p.khs * h + 16 * q4;
+#pragma unroll
+      for (int s = 0; s < 4; s++) qf[nb][s] = *(const f16x8 *)(q + 64 * (s >> 1) + 8 * (s & 1));
+      kmax[nb] = t + 1 < w.end ? t + 1 : w.end;
+      wlo[nb] = p.window && t >= p.window ? t + 1 - p.window : 0u;
+    }
+    clear();
+    float svc = 1.0f;                                                             // what O is held in units of
+    const float sl2 = CAP ? p.scale : p.scale * 1.4426950408889634f;
+
+    auto unit_of = [&](uint32_t i) { return i < w.su ? i : i - w.su + w.lo; };
+    // one unit: scores, softmax, products. kf(tt, s), vf(d): the A operands; then(): once the keys are used
+    auto step = [&](uint32_t un, float sk, float sv, bool none, auto kf, auto then, auto vf) {
+      const uint32_t k0 = un * 32;
+      f32x4 s[NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; nb++) s[nb][0] = s[nb][1] = (f32x4){};
+#pragma unroll
+      for (int tt = 0; tt < 2; tt++)
+#pragma unroll
+        for (int st = 0; st < 4; st++) {
+          const f16x8 ka = kf(tt, st);
+#pragma unroll
+          for (int nb = 0; nb < NB; nb++) s[nb][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qf[nb][st], s[nb][tt], 0, 0, 0);
+        }
+      then();
+      const float f = sk * sl2;
+      f16x8 pb[NB];
+      const float ratio = svc / sv;
+      svc = sv;
+#pragma unroll
+      for (int nb = 0; nb < NB; nb++) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          x[i] = s[nb][i >> 2][i & 3] * f;
+          if constexpr (CAP) x[i] = p.cap * 1.4426950408889634f * (2.0f * sigmoid(2.0f * x[i] / p.cap) - 1.0f);
+        }
+        if (none || __any(k0 + 32 > kmax[nb] || (k0 < wlo[nb] && k0 + 32 > p.sinks))) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const uint32_t j = k0 + 16 * (i >> 2) + 4 * q4 + (i & 3);
+            x[i] = !none && j < kmax[nb] && (j >= wlo[nb] || j < p.sinks) ? x[i] : -1.0e30f;
+          }
+        }
+        float mx = x[0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) mx = fmaxf(mx, x[i]);
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        // the maximum that the exponents subtract moves only when it is passed by more than 8 (P <= 256)
+        const float mn = __any(mx > m[nb] + 8.0f) ? fmaxf(m[nb], mx) : m[nb];
+        const float mns = mn <= -1.0e29f ? 0.0f : mn;
+        float ps = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          x[i] = __builtin_amdgcn_exp2f(x[i] - mns);
+          ps += x[i];
+        }
+        const float al = __builtin_amdgcn_exp2f(m[nb] - mn);
+        l[nb] = l[nb] * al + ps;
+        m[nb] = mn;
+        const float g = al * ratio;
+        if (__any(g != 1.0f)) {
+#pragma unroll
+          for (int d = 0; d < 8; d++) acc[nb][d] *= g;
+        }
+        pb[nb] = (f16x8){(f16)x[0], (f16)x[1], (f16)x[2], (f16)x[3], (f16)x[4], (f16)x[5], (f16)x[6], (f16)x[7]};
+      }
+#pragma unroll
+      for (int d = 0; d < 8; d++) {
+        const f16x8 va = vf(d);
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) acc[nb][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[nb], acc[nb][d], 0, 0, 0);
+      }
+    };
+
+    // whole blocks, up to 64 units ahead: lane i knows unit c0 + i's page and scales
+    constexpr uint32_t NONE = 0xffffffffu;
+    const uint32_t ic = i1 < w.io ? i1 : w.io;
+    for (uint32_t c0 = i0; c0 < ic; c0 += 64) {
+      const uint32_t nc = ic - c0 < 64 ? ic - c0 : 64;
+      uint32_t pg = NONE;
+      float lsk = 1.0f, lsv = 1.0f;
+      if (lane < nc) {
+        const uint32_t un = unit_of(c0 + lane);
+        if (un * 32 < w.end) pg = kv_page(p, w.s.slot, un >> 1);
+        if (pg != NONE) {
+          const f32x2 sc = *(const f32x2 *)(p.scales + kv_scale_at(p, pg, hk, 0));
+          lsk = sc.x;
+          lsv = sc.y;
+        }
+      }
+      // (a unit's keys are asked for when the scores of the one before it are done, its values when that one's are)
+      u32x4 kc[4], vc[4];
+      auto load = [&](uint32_t i, uint32_t kv, u32x4 *to) {
+        const uint32_t g = __builtin_amdgcn_readlane(pg, i), un = unit_of(c0 + i);
+        const uint8_t *c = p.codes + kv_code_at(p, g != NONE ? g : 0u, hk, kv) + (un & 1) * (KV_HEAD / 2) + lane * 16;
+#pragma unroll
+        for (int j = 0; j < 4; j++) to[j] = __builtin_nontemporal_load((const u32x4 *)(c + 1024 * j));
+      };
+      load(0, 0, kc);
+      load(0, 1, vc);
+      for (uint32_t i = 0; i < nc; i++) {
+        const bool more = i + 1 < nc;
+        step(unit_of(c0 + i), rlf(lsk, i), rlf(lsv, i), __builtin_amdgcn_readlane(pg, i) == NONE,
+             [&](int tt, int s) { return kv_f16x8(kc[2 * tt + (s >> 1)][2 * (s & 1)], kc[2 * tt + (s >> 1)][2 * (s & 1) + 1]); },
+             [&] { if (more) load(i + 1, 0, kc); },
+             [&](int d) { return kv_f16x8(vc[d >> 1][2 * (d & 1)], vc[d >> 1][2 * (d & 1) + 1]); });
+        if (more) load(i + 1, 1, vc);
+      }
+    }
+    // the open block, in f16
+    for (uint32_t i = i0 < w.io ? w.io : i0; i < i1; i++) {
+      const uint32_t un = unit_of(i);
+      const u16 *kt = p.tail + kv_tail_at(p, w.s.slot, un >> 1, hk, 0) + (un & 1) * (KV_HEAD / 2) + lane * 8, *vt = kt + KV_HEAD;
+      step(un, 1.0f, 1.0f, false, [&](int tt, int s) { return *(const f16x8 *)(kt + 512 * (4 * tt + s)); }, [] {},
+           [&](int d) {
+             f16x8 v = *(const f16x8 *)(vt + 512 * d);
+#pragma unroll
+             for (int j = 0; j < 8; j++) v[j] = un * 32 + 16 * (j >> 2) + 4 * q4 + (j & 3) < w.end ? v[j] : (f16)0.0f;
+             return v;
+           });
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+#pragma unroll
+      for (int d = 0; d < 8; d++) acc[nb][d] *= svc;
+      l[nb] += __shfl_xor(l[nb], 16, 64);
+      l[nb] += __shfl_xor(l[nb], 32, 64);
+    }
+    u = g0 + i1;
+    if (g0 < a) {                                                                 // another wave began it
+#pragma unroll
+      for (int nb = 0; nb < NB; nb++) {
+#pragma unroll
+        for (int d = 0; d < 8; d++) *(f32x4 *)&sO[wave][((nb * 8 + d) * 64 + lane) * 4] = acc[nb][d];
+        sM[wave][nb * 64 + lane] = m[nb];
+        sL[wave][nb * 64 + lane] = l[nb];
+      }
+    } else if (g0 + w.units > e) {
+      tail = true;
+    } else {
+      put(w, hk, rb);
+    }
+  }
+  __syncthreads();
+
+  // ---- groups that waves share: added to the registers, in order, from wave `from` on; true: the group ended there
+  auto gather = [&](uint32_t from, uint32_t gend) {
+    for (uint32_t v = from; v < (uint32_t)NW && wfirst(v) < wfirst(v + 1); v++) {
+      if (wfirst(v) >= gend) return;
+#pragma unroll
+      for (int nb = 0; nb < NB; nb++) {
+        const float m2 = sM[v][nb * 64 + lane], mn = fmaxf(m[nb], m2);
+        const float f1 = __builtin_amdgcn_exp2f(m[nb] - mn), f2 = __builtin_amdgcn_exp2f(m2 - mn);
+        l[nb] = l[nb] * f1 + sL[v][nb * 64 + lane] * f2;
+        m[nb] = mn;
+#pragma unroll
+        for (int d = 0; d < 8; d++) acc[nb][d] = acc[nb][d] * f1 + *(const f32x4 *)&sO[v][((nb * 8 + d) * 64 + lane) * 4] * f2;
+      }
+    }
+  };
+  if (tail) {
+    gather(wave + 1, g0 + w.units);
+    if (g0 + w.units <= we) put(w, hk, rb);
+    else leave(w, b, hk, rb, g0, 1);
+  }
+  if (wave == 0) {
+    // the group that an earlier workgroup began
+    uint32_t base0;
+    const uint32_t b1 = rfl(find(wa, &base0));
+    const KvWork w1 = kv_work<RB>(p, b1);
+    const uint32_t gi = rfl((wa - base0) / w1.units), g1 = base0 + gi * w1.units;
+    if (g1 < wa) {
+      clear();
+      gather(0, g1 + w1.units);
+      const uint32_t hk1 = rfl(gi / w1.blocks);
+      leave(w1, b1, hk1, gi - hk1 * w1.blocks, g1, 0);
+    }
+  }
+  __syncthreads();
+
+  // ---- groups that workgroups share, whose last part came from here: threads share a row's four d over the parts
+  for (int jb = 0; jb < 2; jb++) {
+    if (!sJob[jb][0]) continue;
+    const uint32_t kf = sJob[jb][1], kl = sJob[jb][2], hk2 = sJob[jb][4], rb2 = sJob[jb][5], np = kl - kf + 1;
+    const KvWork w2 = kv_work<RB>(p, sJob[jb][3]);
+    const uint32_t left = w2.s.n * rep - rb2 * RB, nrow = left < RB ? left : RB, items = nrow * 32;
+    uint32_t sh = 1;                                                              // threads for each item
+    while (sh < 16 && items * sh * 2 <= 64 * NW && sh * 4 <= np) sh *= 2;
+    for (uint32_t it0 = 0; it0 < items; it0 += 64 * NW) {                         // (one pass where sh > 1)
+      const uint32_t it = sh > 1 ? tid % items : it0 + tid, pi = sh > 1 ? tid / items : 0u;
+      const bool live = pi < sh && it < items;
+      const uint32_t r = it >> 5, d = (it & 31u) * 4;
+      float M = -1.0e30f, L = 0.0f;
+      f32x4 o = (f32x4){};
+      if (live) {
+        for (uint32_t s = np * pi / sh, se = np * (pi + 1) / sh; s < se; s += 8) {
+          f32x4 ov[8];
+          f32x2 ml[8];
+#pragma unroll
+          for (uint32_t x = 0; x < 8; x++) {
+            const uint32_t i = s + x < se ? s + x : se - 1u, at = (2 * (kf + i) + (i == 0 ? 1u : 0u)) * PART;
+            ml[x] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(pr, (int)((at + RB * KV_D + 2 * r) * 4u), 0, SC0_SC1));
+            ov[x] = __builtin_bit_cast(f32x4, sys_load128(pr, (at + r * KV_D + d) * 4u));
+          }
+          float Mn = M;
+#pragma unroll
+          for (uint32_t x = 0; x < 8; x++) Mn = fmaxf(Mn, ml[x].x);
+          const float f0 = __builtin_amdgcn_exp2f(M - Mn);
+          o *= f0;
+          L *= f0;
+#pragma unroll
+          for (uint32_t x = 0; x < 8; x++) {
+            const float f = s + x < se ? __builtin_amdgcn_exp2f(ml[x].x - Mn) : 0.0f;
+            o += f * ov[x];
+            L += f * ml[x].y;
+          }
+          M = Mn;
+        }
+      }
+      if (sh > 1) {
+        float *so = &sO[0][0];                                                    // (the waves have taken theirs: the barrier above)
+        __syncthreads();
+        if (live) {
+          *(f32x4 *)(so + (pi * items + it) * 4) = o;
+          *(f32x2 *)(so + 64 * NW * 4 + (pi * items + it) * 2) = (f32x2){M, L};
+        }
+        __syncthreads();
+        if (pi == 0 && live) {
+          for (uint32_t q = 1; q < sh; q++) {
+            const f32x2 ml = *(const f32x2 *)(so + 64 * NW * 4 + (q * items + it) * 2);
+            const float Mn = fmaxf(M, ml.x), fa = __builtin_amdgcn_exp2f(M - Mn), fb = __builtin_amdgcn_exp2f(ml.x - Mn);
+            o = fa * o + fb * *(const f32x4 *)(so + (q * items + it) * 4);
+            L = fa * L + fb * ml.y;
+            M = Mn;
+          }
+        }
+        __syncthreads();
+      }
+      if (live && pi == 0) {
+        const uint32_t row = rb2 * RB + r, qi = row / rep, h = hk2 * rep + (row - qi * rep);
+        const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+        *(u32x2 *)(p.Ko + (uint64_t)(w2.s.r0 + qi) * p.ldo + h * KV_D + d) = (u32x2){pack2(o.x * inv, o.y * inv), pack2(o.z * inv, o.w * inv)};
+      }
+    }
+    if (tid == 0) __hip_atomic_store(cnt + kf, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  }
+}
+
+constexpr int KVA_WG = 2;                         // workgroups for each CU at most
+uint64_t kv_attention_part_bytes(int cus) {
+  return std::max((uint64_t)cus * KVA_WG * 2 * kva_part(32), (uint64_t)cus * 2 * kva_part(64)) * sizeof(float);
+}
+unsigned kv_attention_counters(int cus) { return (unsigned)cus * KVA_WG; }
+
+hipError_t launch_kv_attention(const KvParams &p, int cus, bool ws, float *part, unsigned *cnt, hipStream_t s) {
   if (p.rows == 0 || p.B == 0 || p.Hq == 0) return hipSuccess;
-  hipLaunchKernelGGL(k_kv_attn_row, dim3(p.rows, p.Hq), dim3(64), 0, s, p);
+  const uint64_t rows = (uint64_t)p.rows * (p.Hq / p.Hkv), per = (rows + p.B - 1) / p.B;
+  auto go = [&](auto kernel, int nw, int wg) { hipLaunchKernelGGL(kernel, dim3(cus * wg), dim3(64 * nw), 0, s, p, ws ? 1u : 0u, part, cnt); };
+  if (per <= 16) p.cap > 0.0f ? go(k_kv_attn_split<1, 8, true>, 8, 2) : go(k_kv_attn_split<1, 8, false>, 8, 2);
+  else if (per <= 32) p.cap > 0.0f ? go(k_kv_attn_split<2, 4, true>, 4, 2) : go(k_kv_attn_split<2, 4, false>, 4, 2);
+  else p.cap > 0.0f ? go(k_kv_attn_split<4, 4, true>, 4, 1) : go(k_kv_attn_split<4, 4, false>, 4, 1);
   return hipGetLastError();
 }
 

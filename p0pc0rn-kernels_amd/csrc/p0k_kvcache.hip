@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256) void k_kv_append(KvParams p) {
       for (int g = 0; g < 2; g++) {
         uint32_t v = 0;
 #pragma unroll
-        for (int j = 0; j < 4; j++) v |= ((uint32_t)kv_code(h_val(x[i][4 * g + j]), sc, ri) & 255u) << (8 * j);
+        for (int j = 0; j < 4; j++) v |= (uint32_t)(kv_code(h_val(x[i][4 * g + j]), sc, ri) + 128) << (8 * j);
         w[2 * i + g] = v;
       }
     if (kv == 0) {
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(256) void k_kv_read(KvParams p) {
     for (int i = 0; i < 4; i++)
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        float v = (float)(int8_t)(w[i >> 1][2 * (i & 1) + (j >> 2)] >> (8 * (j & 3))) * sc;
+        const float v = ((float)((w[i >> 1][2 * (i & 1) + (j >> 2)] >> (8 * (j & 3))) & 255u) - 128.0f) * sc;
         x[i][j] = __builtin_bit_cast(uint16_t, (f16)v);
       }
   }

@@ -78,6 +78,9 @@ struct p0k_ctx {
   // partial rows and counters of attention over runs of keys: a fixed size, allocated with the context
   float *ws_attn = nullptr;
   uint32_t *ws_attn_cnt = nullptr;
+  // the same of attention over the 8-bit cache
+  float *ws_kv = nullptr;
+  uint32_t *ws_kv_cnt = nullptr;
   // the id of the capture that p0k_graph_begin began, 0: none (its graphs replay in order with the context's work, so
   // calls in them may use workspaces; a capture begun by the caller may replay anywhere). An id and not a flag: the
   // caller may end that capture with the HIP API and begin one of its own
@@ -130,10 +133,16 @@ int p0k_ctx_create(int device, p0k_ctx **out) {
   if (e == hipSuccess) e = hipMalloc((void **)&c->ws_attn, p0k::attention_part_bytes((int)c->tune.cus));
   if (e == hipSuccess) e = hipMalloc((void **)&c->ws_attn_cnt, sizeof(uint32_t) * p0k::ATTN_COUNTERS);
   if (e == hipSuccess) e = hipMemset(c->ws_attn_cnt, 0, sizeof(uint32_t) * p0k::ATTN_COUNTERS);
+  const uint64_t kv_cnt = sizeof(uint32_t) * p0k::kv_attention_counters((int)c->tune.cus);
+  if (e == hipSuccess) e = hipMalloc((void **)&c->ws_kv, p0k::kv_attention_part_bytes((int)c->tune.cus));
+  if (e == hipSuccess) e = hipMalloc((void **)&c->ws_kv_cnt, kv_cnt);
+  if (e == hipSuccess) e = hipMemset(c->ws_kv_cnt, 0, kv_cnt);
   if (e == hipSuccess) e = hipStreamSynchronize(nullptr);   // the clears are not in order with the context's stream
   if (e != hipSuccess) {
     if (c->ws_attn) (void)hipFree(c->ws_attn);
     if (c->ws_attn_cnt) (void)hipFree(c->ws_attn_cnt);
+    if (c->ws_kv) (void)hipFree(c->ws_kv);
+    if (c->ws_kv_cnt) (void)hipFree(c->ws_kv_cnt);
     if (c->ws_cnt) (void)hipFree(c->ws_cnt);
     if (c->ws_zero) (void)hipFree(c->ws_zero);
     (void)hipStreamDestroy(c->stream);
@@ -164,6 +173,8 @@ void p0k_ctx_destroy(p0k_ctx *c) {
   if (c->ws_x) (void)hipFree(c->ws_x);
   if (c->ws_attn) (void)hipFree(c->ws_attn);
   if (c->ws_attn_cnt) (void)hipFree(c->ws_attn_cnt);
+  if (c->ws_kv) (void)hipFree(c->ws_kv);
+  if (c->ws_kv_cnt) (void)hipFree(c->ws_kv_cnt);
   if (c->ws_zero) (void)hipFree(c->ws_zero);
   if (c->ws_cnt) (void)hipFree(c->ws_cnt);
   for (void *p : c->ws_retired) (void)hipFree(p);
@@ -987,7 +998,11 @@ int p0k_kv_attention(p0k_ctx *c, const p0k_kv_attn_args *a) {
     return r;
   HIPCHK(hipSetDevice(c->device), "hipSetDevice");
   std::lock_guard<std::mutex> order(c->enq);
-  hipError_t e = p0k::launch_kv_attention(p, c->stream);
+  bool capturing, ws;
+  if (int rr = ws_allowed(c, &capturing, &ws)) return rr;
+  if (ws) c->capture_ws = true;
+  const int cus = [&] { std::lock_guard<std::mutex> lk(c->mu); return (int)c->tune.cus; }();
+  hipError_t e = p0k::launch_kv_attention(p, cus, ws, c->ws_kv, c->ws_kv_cnt, c->stream);
   if (e != hipSuccess) return hip_err(e, "kv_attention launch");
   return P0K_OK;
 }
