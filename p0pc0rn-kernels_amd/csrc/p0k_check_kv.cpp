@@ -135,7 +135,8 @@ int prepare_kv_attention(const p0k_kv_attn_args *a, KvParams *out, std::string *
   CHECK(check_cache(err, "kv_attention", a->cache, o.B, o.slot != nullptr, &o));
   NEED(a->Hq > 0 && a->Hq <= 65535u && a->Hq % o.Hkv == 0, "kv_attention: Hq %u is not a multiple of Hkv %u (or too large)", a->Hq, o.Hkv);
   NEED(a->sinks == 0 || a->window != 0, "kv_attention: sinks without a window");
-  NEED(std::isfinite(a->scale) && a->scale >= 0.0f, "kv_attention: scale must be positive (0: 1 / sqrt(128))");
+  // (a masked score is -1e30 before it is scaled, and has to stay far below the others)
+  NEED(a->scale == 0.0f || (a->scale >= 0x1p-40f && a->scale <= 0x1p40f), "kv_attention: scale must be in [2^-40, 2^40] (0: 1 / sqrt(128))");
   NEED(std::isfinite(a->cap) && a->cap >= 0.0f, "kv_attention: cap must be positive (0: none)");
   CHECK(check_heads(err, "kv_attention", "q", a->q_buf, a->q_off, a->q_size, a->q_rs, a->q_hs, o.rows, a->Hq, false, &o.krs, &o.khs));
   NEED(a->o_buf != nullptr, "kv_attention: missing o buffer");
@@ -143,8 +144,9 @@ int prepare_kv_attention(const p0k_kv_attn_args *a, KvParams *out, std::string *
   NEED(a->o_off % 8 == 0 && o.ldo % 4 == 0 && o.ldo >= a->Hq * 128,
        "kv_attention: o offset 8-byte aligned, ldo a multiple of 4 covering Hq * 128");
   if (o.rows) CHECK(fits(err, "kv_attention", "o", a->o_off, ((uint64_t)(o.rows - 1) * o.ldo + a->Hq * 128) * 2, a->o_size));
-  // the kernels count (unit of 32 tokens, head, 16 rows) in 32 bits
-  NEED((unsigned __int128)a->cache.max_pages * 2 * o.Hkv * ((uint64_t)o.rows * (a->Hq / o.Hkv) / 16 + o.B) < (1ull << 32),
+  // the kernels count (unit of 32 tokens, head, 16 rows) in 32 bits, and a launch has fewer than 2^32 threads
+  NEED((unsigned __int128)a->cache.max_pages * 2 * o.Hkv * ((uint64_t)o.rows * (a->Hq / o.Hkv) / 16 + o.B) < (1ull << 32) &&
+           (uint64_t)o.Hkv * ((uint64_t)o.rows * (a->Hq / o.Hkv) / 128 + o.B) < (1ull << 23),
        "kv_attention: max_pages %u with %u rows of %u heads is too large for one call", a->cache.max_pages, o.rows, a->Hq);
   o.K = (const uint16_t *)((const uint8_t *)a->q_buf + a->q_off);
   o.Ko = (uint16_t *)((uint8_t *)a->o_buf + a->o_off);

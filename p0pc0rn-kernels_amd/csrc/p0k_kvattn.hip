@@ -10,6 +10,14 @@ namespace p0k {
 
 typedef unsigned short u16;
 
+// Two results as f16. A mean of cached values is at most 65504, but the rounding of the probabilities can carry it to where
+// f16 rounds to infinity (NaN, of a query's own, stays).
+__device__ __forceinline__ uint32_t pack_o(float a, float b) {
+  a = fabsf(a) < 65600.0f ? fminf(fmaxf(a, -65504.0f), 65504.0f) : a;
+  b = fabsf(b) < 65600.0f ? fminf(fmaxf(b, -65504.0f), 65504.0f) : b;
+  return pack2(a, b);
+}
+
 // What a sequence asks of the kernel: units of 32 tokens, those of the sinks [0, su) and then from unit `lo` on (0 units:
 // nothing to do; a sequence that sees nothing has one that is all masked, for its rows have to be written)
 struct KvWork { KvSeq s; uint32_t end, su, lo, units, blocks, io; };   // io: the first unit of the open block, by its place
@@ -150,7 +158,7 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 4 : NB == 2 ? 2 : 1) void k_kv_a
       u16 *o = p.Ko + (uint64_t)(w.s.r0 + qi) * p.ldo + h * KV_D + 4 * q4;
 #pragma unroll
       for (int d = 0; d < 8; d++)
-        *(u32x2 *)(o + 16 * d) = (u32x2){pack2(acc[nb][d].x * inv, acc[nb][d].y * inv), pack2(acc[nb][d].z * inv, acc[nb][d].w * inv)};
+        *(u32x2 *)(o + 16 * d) = (u32x2){pack_o(acc[nb][d].x * inv, acc[nb][d].y * inv), pack_o(acc[nb][d].z * inv, acc[nb][d].w * inv)};
     }
   };
   const srsrc pr = stream_rsrc((const uint8_t *)part);
@@ -447,10 +455,249 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 4 : NB == 2 ? 2 : 1) void k_kv_a
       if (live && pi == 0) {
         const uint32_t row = rb2 * RB + r, qi = row / rep, h = hk2 * rep + (row - qi * rep);
         const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-        *(u32x2 *)(p.Ko + (uint64_t)(w2.s.r0 + qi) * p.ldo + h * KV_D + d) = (u32x2){pack2(o.x * inv, o.y * inv), pack2(o.z * inv, o.w * inv)};
+        *(u32x2 *)(p.Ko + (uint64_t)(w2.s.r0 + qi) * p.ldo + h * KV_D + d) = (u32x2){pack_o(o.x * inv, o.y * inv), pack_o(o.z * inv, o.w * inv)};
       }
     }
     if (tid == 0) __hip_atomic_store(cnt + kf, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  }
+}
+
+// ---------------------------------------------------------------------------------------- many queries
+// A workgroup owns RB = 32 NW rows of one kv head (a row: one query of one of its Hq / Hkv heads, the heads of a query side by
+// side) and walks their keys, block by block: the codes come into registers two blocks ahead, become f16 on their way into
+// LDS once for all of the rows, and every wave multiplies its 32 rows with them as k_attention does: S^T = K Q^T and O^T +=
+// V^T P as 32x32x16 products, a lane owning a row. The cache's order of tokens is that of the score registers, so V^T needs no
+// transposing read. The keys' scale multiplies the scores. The values' scale goes into the exponent: O is held in units of
+// `ref`, which moves (and O with it) only when a block's scale leaves [ref, 64 ref].
+template <int NW, bool CAP>
+__global__ __launch_bounds__(64 * NW, 2) void k_kv_attn_block(KvParams p, uint32_t items) {
+  constexpr uint32_t RB = 32 * NW, NP = 512 / (64 * NW);                          // pieces of 16 codes a thread moves, keys and values each
+  __shared__ __attribute__((aligned(16))) f16 sK[2][KV_HEAD], sV[2][KV_HEAD];     // [8 d][token], [32 tokens][group][d]: pieces of 8
+  const uint32_t tid = threadIdx.x, lane = tid & 63, gh = lane >> 5, l32 = lane & 31, wave = rfl(tid >> 6);
+  const uint32_t rep = p.Hq / p.Hkv;
+  // kv heads go round the XCDs, so that a head's codes stay in one L2; the longest (last) blocks first
+  const uint32_t hk = blockIdx.x % p.Hkv, item = items - 1 - blockIdx.x / p.Hkv;
+  auto base_of = [&](uint32_t b) { return (uint32_t)((uint64_t)kv_row0(p.cu, b, p.rows) * rep / RB) + b; };
+  uint32_t b = 0;
+  {
+    uint32_t n = p.B;
+    while (n > 1) {
+      const uint32_t st = (n + 63u) / 64u, off = lane * st;
+      const uint64_t m = __ballot(off < n && base_of(b + off) <= item);
+      const uint32_t j = m ? 63u - (uint32_t)__builtin_clzll(m) : 0u;
+      b += j * st;
+      n = n - j * st < st ? n - j * st : st;
+    }
+    b = rfl(b);
+  }
+  const KvSeq s = kv_seq(p, b);
+  const uint32_t ib = base_of(b), rows = s.n * rep;
+  if (item < ib || (item - ib) * RB >= rows) return;
+  const uint32_t row0 = (item - ib) * RB, cap = p.max_pages * KV_T;
+  const uint32_t end = s.ok ? (s.pos + s.n < cap ? s.pos + s.n : cap) : 0u;
+  const uint32_t rlast = row0 + RB - 1 < rows ? row0 + RB - 1 : rows - 1;
+  const uint32_t ta = s.pos + row0 / rep, tb = s.pos + rlast / rep;               // the block's first and last query
+  const uint32_t stop = tb + 1 < end ? tb + 1 : end, all = (stop + KV_T - 1) / KV_T;
+  uint32_t lo = 0, su = 0;
+  if (p.window && ta >= p.window) {
+    const uint32_t l0 = (ta + 1 - p.window) / KV_T, s0 = p.sinks / KV_T + (p.sinks % KV_T != 0u);
+    lo = l0 < all ? l0 : all;
+    su = s0 < lo ? s0 : lo;
+  }
+  const uint32_t nt = su + (all - lo);                                            // tiles: [0, su), [lo, all)
+  auto tile_of = [&](uint32_t i) { return i < su ? i : i - su + lo; };
+
+  uint32_t row = row0 + wave * 32 + l32;
+  const bool live = row < rows;
+  row = live ? row : rows - 1;
+  const uint32_t qi = row / rep, h = hk * rep + (row - qi * rep), t = s.pos + qi;
+  f16x8 qf[8];
+  {
+    const u16 *q = p.K + p.krs * (s.r0 + qi) + p.khs * h + 8 * gh;
+#pragma unroll
+    for (int st = 0; st < 8; st++) qf[st] = *(const f16x8 *)(q + 16 * st);
+  }
+  const uint32_t kmax = t + 1 < end ? t + 1 : end, wlo = p.window && t >= p.window ? t + 1 - p.window : 0u;
+
+  // ---- moving a tile: lane i of every wave knows tile c0 + i's page and scales
+  constexpr uint32_t NONE = 0xffffffffu, OPEN = 0xfffffffeu;
+  uint32_t pg = NONE;
+  float lsk = 1.0f, lsv = 1.0f;
+  auto know = [&](uint32_t c0) {
+    pg = NONE;
+    lsk = lsv = 1.0f;
+    if (c0 + lane < nt) {
+      const uint32_t tl = tile_of(c0 + lane);
+      pg = tl == end / KV_T ? OPEN : kv_page(p, s.slot, tl);
+      if (pg < OPEN) {
+        const f32x2 sc = *(const f32x2 *)(p.scales + kv_scale_at(p, pg, hk, 0));
+        lsk = sc.x;
+        lsv = sc.y;
+      }
+    }
+  };
+  u32x4 ck[NP], cv[NP];
+  uint32_t cg = NONE;                                                             // the page of the tile that they hold
+  auto ask = [&](uint32_t i) {                                                    // codes of tile i into registers
+    cg = __builtin_amdgcn_readlane(pg, i & 63);
+    if (cg < OPEN) {
+      const uint8_t *c = p.codes + kv_code_at(p, cg, hk, 0) + tid * 16;
+#pragma unroll
+      for (uint32_t j = 0; j < NP; j++) {
+        ck[j] = *(const u32x4 *)(c + j * 64 * NW * 16);
+        cv[j] = *(const u32x4 *)(c + KV_HEAD + j * 64 * NW * 16);
+      }
+    }
+  };
+  auto store = [&](uint32_t i, uint32_t bf) {                                     // and as f16 into LDS
+    if (cg < OPEN) {
+#pragma unroll
+      for (uint32_t j = 0; j < NP; j++) {
+        const uint32_t pc = tid + 64 * NW * j, r = pc & 15, q = (pc >> 4) & 3, k = 8 * ((pc >> 6) & 1) + 2 * q, tok = 16 * (pc >> 7) + r;
+        *(f16x8 *)&sK[bf][(k * 64 + tok) * 8] = kv_f16x8(ck[j].x, ck[j].y);
+        *(f16x8 *)&sK[bf][((k + 1) * 64 + tok) * 8] = kv_f16x8(ck[j].z, ck[j].w);
+        const uint32_t g = 4 * (pc >> 8) + q, d = 32 * ((pc >> 6) & 3) + r;
+        *(f16x8 *)&sV[bf][(g * 128 + d) * 8] = kv_f16x8(cv[j].x, cv[j].y);
+        *(f16x8 *)&sV[bf][(g * 128 + d + 16) * 8] = kv_f16x8(cv[j].z, cv[j].w);
+      }
+    } else {
+      const uint32_t tl = tile_of(i);
+      const u16 *kt = p.tail + kv_tail_at(p, s.slot, tl, hk, 0);
+      for (uint32_t pc = tid; pc < 1024; pc += 64 * NW) {
+        const uint32_t r = pc & 15, q = (pc >> 4) & 3, st = (pc >> 6) & 3, tok = 16 * (pc >> 8) + r;
+        f16x8 k = (f16x8){}, v = (f16x8){};
+        const uint32_t tv = tl * KV_T + 32 * (pc >> 9) + 4 * q;                   // V: piece pc = [half][16 d][group][d % 16]
+        if (cg == OPEN) {
+          k = *(const f16x8 *)(kt + pc * 8);
+          v = *(const f16x8 *)(kt + KV_HEAD + pc * 8);
+#pragma unroll
+          for (uint32_t j = 0; j < 8; j++) v[j] = tv + 16 * (j >> 2) + (j & 3) < end ? v[j] : (f16)0.0f;
+        }
+        *(f16x8 *)&sK[bf][((8 * (st >> 1) + 2 * q + (st & 1)) * 64 + tok) * 8] = k;
+        *(f16x8 *)&sV[bf][((4 * (pc >> 9) + q) * 128 + 16 * ((pc >> 6) & 7) + r) * 8] = v;
+      }
+    }
+  };
+
+  f32x16 oacc[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) oacc[i] = (f32x16){};
+  float m = -1.0e30f, l = 0.0f, ref = 0.0f;                                       // ref 0: none yet
+  const float sl2 = CAP ? p.scale : p.scale * 1.4426950408889634f;
+  uint32_t gc = NONE;
+  float sk = 1.0f, sv = 1.0f, skn = 1.0f, svn = 1.0f;
+  if (nt) {
+    know(0);
+    ask(0);
+    store(0, 0);
+    gc = cg;
+    sk = rlf(lsk, 0);
+    sv = rlf(lsv, 0);
+    if (nt > 1) ask(1);
+  }
+  for (uint32_t i = 0; i < nt; i++) {
+    const uint32_t bf = i & 1;
+    __syncthreads();                                                              // tile i is there, tile i - 1 is done with
+    const uint32_t gi = gc;
+    if (i + 1 < nt) {
+      store(i + 1, bf ^ 1);
+      gc = cg;
+      skn = rlf(lsk, (i + 1) & 63);
+      svn = rlf(lsv, (i + 1) & 63);
+      if (i + 2 < nt) {
+        if (((i + 2) & 63) == 0) know(i + 2);
+        ask(i + 2);
+      }
+    }
+    f32x16 sacc[2];
+    sacc[0] = (f32x16){};
+    sacc[1] = (f32x16){};
+#pragma unroll
+    for (int st = 0; st < 8; st++)
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++) {
+        const f16x8 a = *(const f16x8 *)&sK[bf][((2 * st + gh) * 64 + 32 * kb + l32) * 8];
+        sacc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qf[st], sacc[kb], 0, 0, 0);
+      }
+    const float f = sk * sl2;
+    const uint32_t k0 = tile_of(i) * KV_T;
+    float sf = f;
+    if constexpr (CAP) {
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) sacc[kb][r] = p.cap * (2.0f * sigmoid(2.0f * sacc[kb][r] * f / p.cap) - 1.0f);
+      sf = 1.4426950408889634f;
+    }
+    if (gi == NONE || __any(k0 + KV_T > kmax || (k0 < wlo && k0 + KV_T > p.sinks))) {
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const uint32_t j = k0 + 32 * kb + 8 * (r >> 2) + 4 * gh + (r & 3);
+          sacc[kb][r] = gi != NONE && j < kmax && (j >= wlo || j < p.sinks) ? sacc[kb][r] : -1.0e30f;
+        }
+    }
+    float mx = -1.0e30f;
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) mx = fmaxf(mx, sacc[kb][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float mxl = mx <= -1.0e29f ? -1.0e30f : mx * sf;
+    const float mn = __any(mxl > m + 8.0f) ? fmaxf(m, mxl) : m;
+    float scale_o = 1.0f;
+    if (sv < ref || sv > 64.0f * ref) {                                           // (uniform)
+      const float nr = 0.125f * sv;
+      scale_o = ref / nr;
+      ref = nr;
+    }
+    const float lr = __builtin_amdgcn_logf(sv / ref);                             // log2; 0 .. 6
+    const float mns = (mn <= -1.0e29f ? 0.0f : mn) - lr;
+    float ps = 0.0f;
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(sacc[kb][r], sf, -mns));
+        sacc[kb][r] = e;
+        ps += e;
+      }
+    if (scale_o != 1.0f || __any(mn != m)) {
+      const float al = __builtin_amdgcn_exp2f(m - mn);
+      l *= al;
+      const float g = al * scale_o;
+#pragma unroll
+      for (int db = 0; db < 4; db++) oacc[db] *= g;
+    }
+    m = mn;
+    l = fmaf(ps, __builtin_amdgcn_exp2f(-lr), l);
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        const f16x8 bp = {(f16)sacc[kb][4 * c + 0], (f16)sacc[kb][4 * c + 1], (f16)sacc[kb][4 * c + 2], (f16)sacc[kb][4 * c + 3],
+                          (f16)sacc[kb][4 * c + 8], (f16)sacc[kb][4 * c + 9], (f16)sacc[kb][4 * c + 10], (f16)sacc[kb][4 * c + 11]};
+#pragma unroll
+        for (int db = 0; db < 4; db++) {
+          const f16x8 av = *(const f16x8 *)&sV[bf][((4 * kb + 2 * c + gh) * 128 + 32 * db + l32) * 8];
+          oacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, bp, oacc[db], 0, 0, 0);
+        }
+      }
+    sk = skn;
+    sv = svn;
+  }
+
+  const float lt = l + __shfl_xor(l, 32, 64);
+  const float inv = lt > 0.0f ? ref / lt : 0.0f;
+  if (live) {
+    u16 *o = p.Ko + (uint64_t)(s.r0 + qi) * p.ldo + h * KV_D + 4 * gh;
+#pragma unroll
+    for (int db = 0; db < 4; db++)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; g4++)
+        *(u32x2 *)(o + 32 * db + 8 * g4) = (u32x2){pack_o(oacc[db][4 * g4] * inv, oacc[db][4 * g4 + 1] * inv),
+                                                  pack_o(oacc[db][4 * g4 + 2] * inv, oacc[db][4 * g4 + 3] * inv)};
   }
 }
 
@@ -464,6 +711,13 @@ hipError_t launch_kv_attention(const KvParams &p, int cus, bool ws, float *part,
   if (p.rows == 0 || p.B == 0 || p.Hq == 0) return hipSuccess;
   const uint64_t rows = (uint64_t)p.rows * (p.Hq / p.Hkv), per = (rows + p.B - 1) / p.B;
   auto go = [&](auto kernel, int nw, int wg) { hipLaunchKernelGGL(kernel, dim3(cus * wg), dim3(64 * nw), 0, s, p, ws ? 1u : 0u, part, cnt); };
+  if (per > 64) {
+    const uint32_t items = (uint32_t)(rows / 256 + p.B);
+    const dim3 grid(items * p.Hkv), block(512);
+    if (p.cap > 0.0f) hipLaunchKernelGGL((k_kv_attn_block<8, true>), grid, block, 0, s, p, items);
+    else hipLaunchKernelGGL((k_kv_attn_block<8, false>), grid, block, 0, s, p, items);
+    return hipGetLastError();
+  }
   if (per <= 16) p.cap > 0.0f ? go(k_kv_attn_split<1, 8, true>, 8, 2) : go(k_kv_attn_split<1, 8, false>, 8, 2);
   else if (per <= 32) p.cap > 0.0f ? go(k_kv_attn_split<2, 4, true>, 4, 2) : go(k_kv_attn_split<2, 4, false>, 4, 2);
   else p.cap > 0.0f ? go(k_kv_attn_split<4, 4, true>, 4, 1) : go(k_kv_attn_split<4, 4, false>, 4, 1);
