@@ -23,9 +23,9 @@ __device__ __forceinline__ uint32_t pack_o(float a, float b) {
 struct KvWork { KvSeq s; uint32_t end, su, lo, units, blocks, io; };   // io: the first unit of the open block, by its place
 
 template <int RB>                                 // rows of a block (a row: one query of one head)
-__device__ __forceinline__ KvWork kv_work(const KvParams &p, uint32_t b) {
+__device__ __forceinline__ KvWork kv_work(const KvParams &p, const KvSeq &s) {
   KvWork w;
-  w.s = kv_seq(p, b);
+  w.s = s;
   const uint32_t cap = p.max_pages * KV_T, U32 = 32;
   w.end = w.s.ok ? (w.s.pos + w.s.n < cap ? w.s.pos + w.s.n : cap) : 0u;
   const uint32_t all = (w.end + U32 - 1) / U32;
@@ -45,14 +45,18 @@ __device__ __forceinline__ KvWork kv_work(const KvParams &p, uint32_t b) {
   return w;
 }
 
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {                       // inclusive prefix sums over the wave
-  const uint32_t lane = threadIdx.x & 63u;
-#pragma unroll
-  for (uint32_t o = 1; o < 64; o <<= 1) {
-    const uint32_t u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
-  }
-  return v;
+// inclusive prefix sums over the wave: within rows of 16 lanes, then their sums onwards
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = dpp_add<0x111, 0xf>(v);                     // row_shr 1, 2, 4, 8
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);                     // row_bcast 15 into rows 1 and 3
+  return dpp_add<0x143, 0xc>(v);                  // row_bcast 31 into rows 2 and 3
 }
 __device__ __forceinline__ uint32_t rfl(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ float rlf(float v, uint32_t l) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), l)); }
@@ -67,52 +71,57 @@ __device__ __forceinline__ float rlf(float v, uint32_t l) { return __uint_as_flo
 // the B operand of the second product, and the cache's layout makes 16-byte loads the A operands of both. Codes are exact
 // in f16; the scales stay in fp32: the keys' multiplies the scores, and O is held in units of the current block's value scale.
 template <int NB, int NW, bool CAP>
-__global__ __launch_bounds__(64 * NW, NB == 1 ? 4 : NB == 2 ? 2 : 1) void k_kv_attn_split(KvParams p, uint32_t ws, float *part, uint32_t *cnt) {
+__global__ __launch_bounds__(64 * NW, NW / 4) void k_kv_attn_split(KvParams p, uint32_t ws, float *part, uint32_t *cnt) {
   constexpr uint32_t RB = 16 * NB, PART = kva_part(RB);
   __shared__ __attribute__((aligned(16))) float sO[NW][NB * 8 * 64 * 4];
   __shared__ float sM[NW][NB * 64], sL[NW][NB * 64];
-  __shared__ uint32_t sJob[2][6];                                                 // groups whose last part this workgroup brought
+  __shared__ uint32_t sJob[2][7];                                                 // groups whose last part this workgroup brought
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = rfl(tid >> 6), r16 = lane & 15, q4 = lane >> 4;
   const uint32_t rep = p.Hq / p.Hkv;
   if (tid < 2) sJob[tid][0] = 0;
 
   // ---- all units, and this workgroup's and wave's share of them
-  uint32_t T = 0, tot0 = 0;
-  for (uint32_t b0 = 0; b0 < p.B; b0 += 64) {
+  // (lane i knows sequence cb + i: what it has, and the units up to its end from the chunk's start)
+  KvSeq ls;
+  uint32_t cb = 0, sum = 0;
+  auto chunk = [&](uint32_t b0) {
+    cb = b0;
+    ls = KvSeq{};
     uint32_t t = 0;
     if (b0 + lane < p.B) {
-      const KvWork w = kv_work<RB>(p, b0 + lane);
+      ls = kv_seq(p, b0 + lane);
+      const KvWork w = kv_work<RB>(p, ls);
       t = w.units * w.blocks * p.Hkv;
     }
-    if (b0 == 0) tot0 = t;
-    T += __builtin_amdgcn_readlane(wave_scan(t), 63);
-  }
-  // the sequence of unit u, and its first unit
-  auto find = [&](uint32_t u, uint32_t *base) {
-    uint32_t at = 0;
-    for (uint32_t b0 = 0; b0 < p.B; b0 += 64) {
-      uint32_t t = tot0;
-      if (b0) {
-        t = 0;
-        if (b0 + lane < p.B) {
-          const KvWork w = kv_work<RB>(p, b0 + lane);
-          t = w.units * w.blocks * p.Hkv;
-        }
-      }
-      const uint32_t sum = wave_scan(t);
-      const uint64_t m = __ballot(at + sum > u);
-      if (m) {
-        const uint32_t f = (uint32_t)__builtin_ctzll(m);
-        *base = at + __builtin_amdgcn_readlane(sum - t, f);
-        return b0 + f;
-      }
-      at += __builtin_amdgcn_readlane(sum, 63);
-    }
-    *base = T;
-    return p.B;
+    sum = wave_scan(t);
+    return __builtin_amdgcn_readlane(sum, 63);
   };
-  uint32_t nwg = gridDim.x;
-  nwg = T < nwg ? T : nwg;
+  auto work = [&](uint32_t b) {                                                   // of sequence b
+    if (b - cb >= 64) chunk(b & ~63u);
+    const uint32_t i = b - cb;
+    KvSeq q;
+    q.r0 = __builtin_amdgcn_readlane(ls.r0, i);
+    q.n = __builtin_amdgcn_readlane(ls.n, i);
+    q.pos = __builtin_amdgcn_readlane(ls.pos, i);
+    q.slot = __builtin_amdgcn_readlane(ls.slot, i);
+    q.ok = __builtin_amdgcn_readlane((uint32_t)ls.ok, i) != 0;
+    return kv_work<RB>(p, q);
+  };
+  uint32_t T = chunk(0);
+  for (uint32_t b0 = 64; b0 < p.B; b0 += 64) T += chunk(b0);
+  // the sequence of unit u < T, and its first unit
+  auto find = [&](uint32_t u, uint32_t *base) {
+    uint32_t at = 0, all = cb == 0 ? __builtin_amdgcn_readlane(sum, 63) : chunk(0);
+    while (at + all <= u) {
+      at += all;
+      all = chunk(cb + 64);
+    }
+    const uint32_t f = (uint32_t)__builtin_ctzll(__ballot(at + sum > u));
+    *base = at + (f ? __builtin_amdgcn_readlane(sum, f - 1) : 0u);
+    return cb + f;
+  };
+  uint32_t nwg = (T + 3) / 4;                                                     // at least 4 units each
+  nwg = nwg < gridDim.x ? nwg : gridDim.x;
   // (row blocks that share their keys go to one XCD)
   const uint32_t blk = blockIdx.x, k = NB > 1 && nwg == gridDim.x && (nwg & 7u) == 0u ? (blk & 7u) * (nwg >> 3) + (blk >> 3) : blk;
   if (k >= nwg) return;
@@ -125,8 +134,7 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 4 : NB == 2 ? 2 : 1) void k_kv_a
     for (int i = 0; i < 2; i++) {
       uint32_t u = i ? we : wa, base;
       if (u < T) {
-        const uint32_t b = rfl(find(u, &base));
-        const KvWork w = kv_work<RB>(p, b);
+        const KvWork w = work(find(u, &base));
         u -= (u - base) % w.units;
       }
       (i ? we : wa) = rfl(u);
@@ -163,7 +171,7 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 4 : NB == 2 ? 2 : 1) void k_kv_a
   };
   const srsrc pr = stream_rsrc((const uint8_t *)part);
   // this block's rows into the workspace; the last workgroup of the group to arrive takes it on (sJob)
-  auto leave = [&](const KvWork &w, uint32_t b, uint32_t hk, uint32_t rb, uint32_t g0, uint32_t out) {
+  auto leave = [&](const KvWork &w, uint32_t hk, uint32_t rb, uint32_t g0, uint32_t out) {
     const uint32_t base = (2 * k + out) * PART;
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
@@ -180,16 +188,18 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 4 : NB == 2 ? 2 : 1) void k_kv_a
     uint32_t old = 0;
     if (lane == 0) old = __hip_atomic_fetch_add(cnt + kf, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
     if (rfl(old) == kl - kf && lane == 0) {
-      sJob[out][0] = 1; sJob[out][1] = kf; sJob[out][2] = kl; sJob[out][3] = b; sJob[out][4] = hk; sJob[out][5] = rb;
+      sJob[out][0] = 1; sJob[out][1] = kf; sJob[out][2] = kl; sJob[out][3] = hk; sJob[out][4] = rb; sJob[out][5] = w.s.r0; sJob[out][6] = w.s.n;
     }
   };
 
   uint32_t u = a, base = 0, b = 0, hk = 0, rb = 0, g0 = 0;
   KvWork w;
   bool tail = false;                                                              // the registers hold a group that goes on
-  if (a < e) b = rfl(find(a, &base));
+  KvWork wi;                                                                      // wave 0: the group that an earlier workgroup began
+  uint32_t hki = 0, rbi = 0, gi0 = wa;
+  if (a < e) b = find(a, &base);
   while (u < e) {
-    w = kv_work<RB>(p, b);
+    w = work(b);
     const uint32_t per_seq = w.units * w.blocks * p.Hkv;
     if (u >= base + per_seq) {                                                    // (sequences without rows have no units)
       base += per_seq;
@@ -200,6 +210,7 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 4 : NB == 2 ? 2 : 1) void k_kv_a
     hk = rfl(gi / w.blocks);
     rb = gi - hk * w.blocks;
     g0 = base + gi * w.units;
+    if (g0 < wa) { wi = w; hki = hk; rbi = rb; gi0 = g0; }
     const uint32_t i0 = u - g0, i1 = (e < g0 + w.units ? e : g0 + w.units) - g0;  // units of the group, by their place in it
 
     // ---- the rows' queries: lane r16 holds row nb * 16 + r16, k step s = (64 d, 8 d) its d 64 (s / 2) + 16 q4 + 8 (s % 2) ..
@@ -377,29 +388,20 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 4 : NB == 2 ? 2 : 1) void k_kv_a
   if (tail) {
     gather(wave + 1, g0 + w.units);
     if (g0 + w.units <= we) put(w, hk, rb);
-    else leave(w, b, hk, rb, g0, 1);
+    else leave(w, hk, rb, g0, 1);
   }
-  if (wave == 0) {
-    // the group that an earlier workgroup began
-    uint32_t base0;
-    const uint32_t b1 = rfl(find(wa, &base0));
-    const KvWork w1 = kv_work<RB>(p, b1);
-    const uint32_t gi = rfl((wa - base0) / w1.units), g1 = base0 + gi * w1.units;
-    if (g1 < wa) {
-      clear();
-      gather(0, g1 + w1.units);
-      const uint32_t hk1 = rfl(gi / w1.blocks);
-      leave(w1, b1, hk1, gi - hk1 * w1.blocks, g1, 0);
-    }
+  if (wave == 0 && gi0 < wa) {
+    clear();
+    gather(0, gi0 + wi.units);
+    leave(wi, hki, rbi, gi0, 0);
   }
   __syncthreads();
 
   // ---- groups that workgroups share, whose last part came from here: threads share a row's four d over the parts
   for (int jb = 0; jb < 2; jb++) {
     if (!sJob[jb][0]) continue;
-    const uint32_t kf = sJob[jb][1], kl = sJob[jb][2], hk2 = sJob[jb][4], rb2 = sJob[jb][5], np = kl - kf + 1;
-    const KvWork w2 = kv_work<RB>(p, sJob[jb][3]);
-    const uint32_t left = w2.s.n * rep - rb2 * RB, nrow = left < RB ? left : RB, items = nrow * 32;
+    const uint32_t kf = sJob[jb][1], kl = sJob[jb][2], hk2 = sJob[jb][3], rb2 = sJob[jb][4], np = kl - kf + 1;
+    const uint32_t r0 = sJob[jb][5], left = sJob[jb][6] * rep - rb2 * RB, nrow = left < RB ? left : RB, items = nrow * 32;
     uint32_t sh = 1;                                                              // threads for each item
     while (sh < 16 && items * sh * 2 <= 64 * NW && sh * 4 <= np) sh *= 2;
     for (uint32_t it0 = 0; it0 < items; it0 += 64 * NW) {                         // (one pass where sh > 1)
@@ -455,7 +457,7 @@ __global__ __launch_bounds__(64 * NW, NB == 1 ? 4 : NB == 2 ? 2 : 1) void k_kv_a
       if (live && pi == 0) {
         const uint32_t row = rb2 * RB + r, qi = row / rep, h = hk2 * rep + (row - qi * rep);
         const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-        *(u32x2 *)(p.Ko + (uint64_t)(w2.s.r0 + qi) * p.ldo + h * KV_D + d) = (u32x2){pack_o(o.x * inv, o.y * inv), pack_o(o.z * inv, o.w * inv)};
+        *(u32x2 *)(p.Ko + (uint64_t)(r0 + qi) * p.ldo + h * KV_D + d) = (u32x2){pack_o(o.x * inv, o.y * inv), pack_o(o.z * inv, o.w * inv)};
       }
     }
     if (tid == 0) __hip_atomic_store(cnt + kf, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
@@ -701,16 +703,14 @@ __global__ __launch_bounds__(64 * NW, 2) void k_kv_attn_block(KvParams p, uint32
   }
 }
 
-constexpr int KVA_WG = 2;                         // workgroups for each CU at most
 uint64_t kv_attention_part_bytes(int cus) {
-  return std::max((uint64_t)cus * KVA_WG * 2 * kva_part(32), (uint64_t)cus * 2 * kva_part(64)) * sizeof(float);
+  return (uint64_t)cus * 2 * kva_part(64) * sizeof(float);
 }
-unsigned kv_attention_counters(int cus) { return (unsigned)cus * KVA_WG; }
+unsigned kv_attention_counters(int cus) { return (unsigned)cus; }
 
 hipError_t launch_kv_attention(const KvParams &p, int cus, bool ws, float *part, unsigned *cnt, hipStream_t s) {
   if (p.rows == 0 || p.B == 0 || p.Hq == 0) return hipSuccess;
   const uint64_t rows = (uint64_t)p.rows * (p.Hq / p.Hkv), per = (rows + p.B - 1) / p.B;
-  auto go = [&](auto kernel, int nw, int wg) { hipLaunchKernelGGL(kernel, dim3(cus * wg), dim3(64 * nw), 0, s, p, ws ? 1u : 0u, part, cnt); };
   if (per > 64) {
     const uint32_t items = (uint32_t)(rows / 256 + p.B);
     const dim3 grid(items * p.Hkv), block(512);
@@ -718,9 +718,10 @@ hipError_t launch_kv_attention(const KvParams &p, int cus, bool ws, float *part,
     else hipLaunchKernelGGL((k_kv_attn_block<8, false>), grid, block, 0, s, p, items);
     return hipGetLastError();
   }
-  if (per <= 16) p.cap > 0.0f ? go(k_kv_attn_split<1, 8, true>, 8, 2) : go(k_kv_attn_split<1, 8, false>, 8, 2);
-  else if (per <= 32) p.cap > 0.0f ? go(k_kv_attn_split<2, 4, true>, 4, 2) : go(k_kv_attn_split<2, 4, false>, 4, 2);
-  else p.cap > 0.0f ? go(k_kv_attn_split<4, 4, true>, 4, 1) : go(k_kv_attn_split<4, 4, false>, 4, 1);
+  auto go = [&](auto kernel, int nw) { hipLaunchKernelGGL(kernel, dim3(cus), dim3(64 * nw), 0, s, p, ws ? 1u : 0u, part, cnt); };
+  if (per <= 16) p.cap > 0.0f ? go(k_kv_attn_split<1, 8, true>, 8) : go(k_kv_attn_split<1, 8, false>, 8);
+  else if (per <= 32) p.cap > 0.0f ? go(k_kv_attn_split<2, 8, true>, 8) : go(k_kv_attn_split<2, 8, false>, 8);
+  else p.cap > 0.0f ? go(k_kv_attn_split<4, 4, true>, 4) : go(k_kv_attn_split<4, 4, false>, 4);
   return hipGetLastError();
 }
 
