@@ -7,6 +7,7 @@
 
 namespace p0k {
 
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
 // f16 bits held to the finite range, NaN to 0
@@ -25,73 +26,103 @@ __device__ __forceinline__ int kv_code(float x, float s, float rs) {
   return (int)c;
 }
 
-// One workgroup takes one block of one sequence and kv head, keys or values: thread (t, c) holds d 16 c .. + 15 and 64 + 16 c
-// .. + 15 of token t, its 32 values in registers, so a row is read once.
-__global__ __launch_bounds__(256) void k_kv_append(KvParams p) {
-  __shared__ __attribute__((aligned(16))) uint8_t sC[KV_T][KV_D + 4];
-  __shared__ float sMax[4];
-  const uint32_t item = blockIdx.x, h = blockIdx.y, kv = blockIdx.z, tid = threadIdx.x;
-  const uint32_t b = kv_item_seq<KV_T>(p, item), base = kv_item_base<KV_T>(p, b);
-  const KvSeq s = kv_seq(p, b);
-  if (item < base || !s.ok || s.n == 0) return;
-  const uint32_t cap = p.max_pages * KV_T, k0 = s.pos / KV_T, blk = k0 + (item - base);
-  const uint32_t end = s.pos + s.n < cap ? s.pos + s.n : cap;
-  if (blk >= p.max_pages || blk * KV_T >= end) return;
-
-  const uint16_t *X = (kv ? p.V : p.K) + (kv ? p.vhs : p.khs) * h;
-  const uint64_t rs = kv ? p.vrs : p.krs;
-  const uint32_t t = tid >> 2, c = tid & 3;
-  u16x8 x[4];                                    // d 16 c, 16 c + 8, 64 + 16 c, 72 + 16 c of token t
-  auto dof = [&](int i) { return 16 * c + (i >> 1) * 64 + (i & 1) * 8; };
-  // the rows of a block that this call brings (true: token t is one)
-  auto fresh = [&](uint32_t block) {
-    const uint32_t tok = block * KV_T + t;
-    const bool is = tok >= s.pos && tok < end;
-    if (is) {
-      const uint16_t *row = X + rs * (s.r0 + (tok - s.pos));
+// One workgroup takes one block of one sequence and kv head, keys or values, and every thread 32 of its values, in
+// registers from the first load to the last store. Keys: token tid / 4, d 16 c .. + 15 and 64 + 16 c .. (c = tid % 4): whole
+// pieces of the cache. Values: tokens 4 (tid / 16) .. + 3, d 8 (tid % 16) .. + 7: the four tokens of a d are a word of a
+// piece, and pieces are put together in LDS.
+template <int KV>
+struct Part {
+  uint32_t tid;
+  __device__ uint32_t tok(int i) const { return KV ? 4 * (tid >> 4) + i : tid >> 2; }                               // token and
+  __device__ uint32_t d(int i) const { return KV ? 8 * (tid & 15) : 16 * (tid & 3) + (i >> 1) * 64 + (i & 1) * 8; }   // first d of x[i]
+  // x from / to the tail, the values whose token passes `is`
+  template <class F>
+  __device__ void load_tail(const uint16_t *tail, u16x8 *x, F is) const {
+    if constexpr (KV == 0) {
+      if (is(tok(0))) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        x[i] = *(const u16x8 *)(row + dof(i));
+        for (int i = 0; i < 4; i++) x[i] = *(const u16x8 *)(tail + kv_ktail(tok(0), d(i)));
+      }
+    } else {
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < 4; i++) any |= is(tok(i));
+      if (!any) return;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const u16x4 w = *(const u16x4 *)(tail + kv_vtail(tok(0), d(0) + j));
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (is(tok(i))) x[i][j] = w[i];
+      }
+    }
+  }
+  template <class F>
+  __device__ void store_tail(uint16_t *tail, const u16x8 *x, F is) const {
+    if constexpr (KV == 0) {
+      if (is(tok(0))) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) *(u16x8 *)(tail + kv_ktail(tok(0), d(i))) = x[i];
+      }
+    } else {
+      bool any = false, all = true;
+#pragma unroll
+      for (int i = 0; i < 4; i++) { any |= is(tok(i)); all &= is(tok(i)); }
+      if (!any) return;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        uint16_t *at = tail + kv_vtail(tok(0), d(0) + j);
+        if (all) {
+          *(u16x4 *)at = (u16x4){x[0][j], x[1][j], x[2][j], x[3][j]};
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (is(tok(i))) at[i] = x[i][j];
+        }
+      }
+    }
+  }
+};
+
+template <int KV>
+__device__ void append_block(const KvParams &p, const KvSeq &s, uint32_t blk, uint32_t k0, uint32_t end, uint32_t h, uint8_t *sC, float *sMax) {
+  const uint32_t tid = threadIdx.x;
+  const Part<KV> part{tid};
+  const uint16_t *X = (KV ? p.V : p.K) + (KV ? p.vhs : p.khs) * h;
+  const uint64_t rs = KV ? p.vrs : p.krs;
+  u16x8 x[4];
+  // the values of a block that this call brings
+  auto fresh = [&](uint32_t block) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t t = block * KV_T + part.tok(i);
+      if (t >= s.pos && t < end) {
+        x[i] = *(const u16x8 *)(X + rs * (s.r0 + (t - s.pos)) + part.d(i));
 #pragma unroll
         for (int j = 0; j < 8; j++) x[i][j] = kv_finite(x[i][j]);
       }
     }
-    return is;
   };
-  auto keep = [&](uint32_t block) {              // token t's values into the tail
-    uint16_t *tail = p.tail + kv_tail_at(p, s.slot, block, h, kv);
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      if (kv == 0) {
-        *(u16x8 *)(tail + kv_ktail(t, dof(i))) = x[i];
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) tail[kv_vtail(t, dof(i) + j)] = x[i][j];
-      }
-    }
+  auto keep = [&](uint32_t block) {              // and into the tail
+    part.store_tail(p.tail + kv_tail_at(p, s.slot, block, h, KV), x, [&](uint32_t t) {
+      const uint32_t tt = block * KV_T + t;
+      return tt >= s.pos && tt < end;
+    });
   };
 #pragma unroll
   for (int i = 0; i < 4; i++) x[i] = (u16x8){};
-  const bool is = fresh(blk), whole = (blk + 1) * KV_T <= end;
+  fresh(blk);
   // The tail keeps the last block and the one before it. Of its two places, the first block's may still be read (the tokens
   // that it held before this call): that block's workgroup writes it, after it has read.
   const uint32_t last = end / KV_T;
-  if (is && blk + 1 >= last && (blk == k0 || ((blk ^ k0) & 1))) keep(blk);
-  if (whole) {
-    const uint32_t tok = blk * KV_T + t;
-    if (tok < s.pos) {
-      const uint16_t *tail = p.tail + kv_tail_at(p, s.slot, blk, h, kv);
+  if (blk + 1 >= last && (blk == k0 || ((blk ^ k0) & 1))) keep(blk);
+  if ((blk + 1) * KV_T <= end) {
+    if (blk * KV_T < s.pos) {
+      part.load_tail(p.tail + kv_tail_at(p, s.slot, blk, h, KV), x, [&](uint32_t t) { return blk * KV_T + t < s.pos; });
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        if (kv == 0) {
-          x[i] = *(const u16x8 *)(tail + kv_ktail(t, dof(i)));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; j++) x[i][j] = tail[kv_vtail(t, dof(i) + j)];
-        }
+      for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int j = 0; j < 8; j++) x[i][j] = kv_finite(x[i][j]);   // (a tail that no call has written)
-      }
     }
     uint32_t mx = 0;                             // |x| as bits: finite f16 order as integers
 #pragma unroll
@@ -105,120 +136,115 @@ __global__ __launch_bounds__(256) void k_kv_append(KvParams p) {
     const float sc = amax > 0.0f ? amax / 127.0f : 1.0f, ri = 1.0f / sc;
     const uint32_t page = kv_page(p, s.slot, blk);
     const bool have = page != 0xffffffffu;
-    uint8_t *codes = p.codes + kv_code_at(p, have ? page : 0u, h, kv);
-    uint32_t w[8];
+    uint8_t *codes = p.codes + kv_code_at(p, have ? page : 0u, h, KV);
+    auto code = [&](uint16_t v) { return (uint32_t)(kv_code(h_val(v), sc, ri) + 128); };
+    if constexpr (KV == 0) {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+      for (int i = 0; i < 2; i++) {
+        u32x4 w;
 #pragma unroll
-      for (int g = 0; g < 2; g++) {
-        uint32_t v = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) v |= (uint32_t)(kv_code(h_val(x[i][4 * g + j]), sc, ri) + 128) << (8 * j);
-        w[2 * i + g] = v;
-      }
-    if (kv == 0) {
-      if (have) {
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-          *(u32x4 *)(codes + kv_kcode(t, 64 * i + 16 * c)) = (u32x4){w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+        for (int g = 0; g < 4; g++) {
+          const u16x8 &v = x[2 * i + (g >> 1)];
+          const int j = 4 * (g & 1);
+          w[g] = code(v[j]) | code(v[j + 1]) << 8 | code(v[j + 2]) << 16 | code(v[j + 3]) << 24;
+        }
+        if (have) *(u32x4 *)(codes + kv_kcode(part.tok(0), part.d(2 * i))) = w;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; i++) *(uint32_t *)&sC[t][16 * c + (i >> 2) * 64 + (i & 3) * 4] = w[i];
+      for (int j = 0; j < 8; j++)
+        *(uint32_t *)(sC + kv_vcode(part.tok(0), part.d(0) + j)) = code(x[0][j]) | code(x[1][j]) << 8 | code(x[2][j]) << 16 | code(x[3][j]) << 24;
       __syncthreads();
       if (have) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const uint32_t pc = tid + 256 * i, tq = 32 * (pc >> 8) + 4 * ((pc >> 4) & 3), d = 32 * ((pc >> 6) & 3) + (pc & 15);
-          u32x4 o;
-#pragma unroll
-          for (int g = 0; g < 4; g++) {          // bytes 4 g ..: d + 16 (g / 2), tokens tq + 16 (g % 2) ..
-            uint32_t v = 0;
-#pragma unroll
-            for (int j = 0; j < 4; j++) v |= (uint32_t)sC[tq + 16 * (g & 1) + j][d + 16 * (g >> 1)] << (8 * j);
-            o[g] = v;
-          }
-          *(u32x4 *)(codes + 16 * pc) = o;
-        }
+        for (int i = 0; i < 2; i++) *(u32x4 *)(codes + 16 * (tid + 256 * i)) = *(const u32x4 *)(sC + 16 * (tid + 256 * i));
       }
     }
-    if (have && tid == 0) p.scales[kv_scale_at(p, page, h, kv)] = sc;
+    if (have && tid == 0) p.scales[kv_scale_at(p, page, h, KV)] = sc;
   }
   if (blk == k0) {
     const uint32_t cb = ((last ^ k0) & 1) ? last - 1 : last;   // the one of the last two in the first block's place
-    if (cb > k0 && cb * KV_T < end && last >= 1) {
+    if (last >= 1 && cb > k0 && cb * KV_T < end) {
       __syncthreads();                           // (the whole workgroup has read the first block's tokens)
-      if (fresh(cb)) keep(cb);
+      fresh(cb);
+      keep(cb);
     }
   }
 }
 
-__global__ __launch_bounds__(256) void k_kv_read(KvParams p) {
-  __shared__ __attribute__((aligned(16))) uint8_t sC[KV_T][KV_D + 4];
-  const uint32_t item = blockIdx.x, h = blockIdx.y, kv = blockIdx.z, tid = threadIdx.x;
+__global__ __launch_bounds__(256) void k_kv_append(KvParams p) {
+  __shared__ __attribute__((aligned(16))) uint8_t sC[KV_HEAD];
+  __shared__ float sMax[4];
+  const uint32_t item = blockIdx.x, h = blockIdx.y;
   const uint32_t b = kv_item_seq<KV_T>(p, item), base = kv_item_base<KV_T>(p, b);
   const KvSeq s = kv_seq(p, b);
-  if (item < base || s.n == 0) return;
-  const uint32_t blk = s.pos / KV_T + (item - base), t = tid >> 2, c = tid & 3, end = s.pos + s.n;
-  if (blk * KV_T >= end) return;
-  const int32_t held = p.len[b];
-  const uint32_t cap = p.max_pages * KV_T, len = !s.ok || held < 0 ? 0u : (uint32_t)held < cap ? (uint32_t)held : cap;
-  const uint32_t tok = blk * KV_T + t;
-  const bool open = blk == len / KV_T;
-  const uint32_t page = open || blk > len / KV_T ? 0xffffffffu : kv_page(p, s.slot, blk);
+  if (item < base || !s.ok || s.n == 0) return;
+  const uint32_t cap = p.max_pages * KV_T, k0 = s.pos / KV_T, blk = k0 + (item - base);
+  const uint32_t end = s.pos + s.n < cap ? s.pos + s.n : cap;
+  if (blk >= p.max_pages || blk * KV_T >= end) return;
+  if (blockIdx.z == 0) append_block<0>(p, s, blk, k0, end, h, sC, sMax);
+  else append_block<1>(p, s, blk, k0, end, h, sC, sMax);
+}
+
+// code * scale of byte j of a word (byte = code + 128; 128 s is exact, so the fma rounds code * s once)
+__device__ __forceinline__ uint16_t kv_value(uint32_t w, int j, float sc) {
+  float v = fmaf((float)((w >> (8 * j)) & 255u), sc, -128.0f * sc);
+  asm volatile("" : "+v"(v));                     // (rounded to fp32 before it is rounded to f16)
+  return __builtin_bit_cast(uint16_t, (f16)v);
+}
+
+template <int KV>
+__device__ void read_block(const KvParams &p, const KvSeq &s, uint32_t blk, uint32_t len, uint32_t h, uint8_t *sC) {
+  const uint32_t tid = threadIdx.x, end = s.pos + s.n;
+  const Part<KV> part{tid};
   u16x8 x[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) x[i] = (u16x8){};
-  auto dof = [&](int i) { return 16 * c + (i >> 1) * 64 + (i & 1) * 8; };
-  if (open) {
-    if (tok < len) {
-      const uint16_t *tail = p.tail + kv_tail_at(p, s.slot, blk, h, kv);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        if (kv == 0) {
-          x[i] = *(const u16x8 *)(tail + kv_ktail(t, dof(i)));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; j++) x[i][j] = tail[kv_vtail(t, dof(i) + j)];
-        }
-      }
-    }
+  const uint32_t page = blk < len / KV_T ? kv_page(p, s.slot, blk) : 0xffffffffu;
+  if (blk == len / KV_T) {
+    part.load_tail(p.tail + kv_tail_at(p, s.slot, blk, h, KV), x, [&](uint32_t t) { return blk * KV_T + t < len; });
   } else if (page != 0xffffffffu) {
-    const uint8_t *codes = p.codes + kv_code_at(p, page, h, kv);
-    const float sc = p.scales[kv_scale_at(p, page, h, kv)];
-    u32x4 w[2];
-    if (kv == 0) {
-#pragma unroll
-      for (int i = 0; i < 2; i++) w[i] = *(const u32x4 *)(codes + kv_kcode(t, 64 * i + 16 * c));
-    } else {
+    const uint8_t *codes = p.codes + kv_code_at(p, page, h, KV);
+    const float sc = p.scales[kv_scale_at(p, page, h, KV)];
+    if constexpr (KV == 0) {
 #pragma unroll
       for (int i = 0; i < 2; i++) {
-        const uint32_t pc = tid + 256 * i, tq = 32 * (pc >> 8) + 4 * ((pc >> 4) & 3), d = 32 * ((pc >> 6) & 3) + (pc & 15);
-        const u32x4 o = *(const u32x4 *)(codes + 16 * pc);
+        const u32x4 w = *(const u32x4 *)(codes + kv_kcode(part.tok(0), part.d(2 * i)));
 #pragma unroll
-        for (int g = 0; g < 4; g++)
-#pragma unroll
-          for (int j = 0; j < 4; j++) sC[tq + 16 * (g & 1) + j][d + 16 * (g >> 1)] = (uint8_t)(o[g] >> (8 * j));
+        for (int j = 0; j < 16; j++) x[2 * i + (j >> 3)][j & 7] = kv_value(w[j >> 2], j & 3, sc);
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; i++) *(u32x4 *)(sC + 16 * (tid + 256 * i)) = *(const u32x4 *)(codes + 16 * (tid + 256 * i));
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) w[i][j] = *(const uint32_t *)&sC[t][64 * i + 16 * c + 4 * j];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
       for (int j = 0; j < 8; j++) {
-        const float v = ((float)((w[i >> 1][2 * (i & 1) + (j >> 2)] >> (8 * (j & 3))) & 255u) - 128.0f) * sc;
-        x[i][j] = __builtin_bit_cast(uint16_t, (f16)v);
-      }
-  }
-  if (tok >= s.pos && tok < end) {
-    uint16_t *row = (kv ? p.Vo : p.Ko) + (kv ? p.vhs : p.khs) * h + (kv ? p.vrs : p.krs) * (s.r0 + (tok - s.pos));
+        const uint32_t w = *(const uint32_t *)(sC + kv_vcode(part.tok(0), part.d(0) + j));
 #pragma unroll
-    for (int i = 0; i < 4; i++) *(u16x8 *)(row + dof(i)) = x[i];
+        for (int i = 0; i < 4; i++) x[i][j] = kv_value(w, i, sc);
+      }
+    }
   }
+  uint16_t *Y = (KV ? p.Vo : p.Ko) + (KV ? p.vhs : p.khs) * h;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t t = blk * KV_T + part.tok(i);
+    if (t >= s.pos && t < end) *(u16x8 *)(Y + (KV ? p.vrs : p.krs) * (s.r0 + (t - s.pos)) + part.d(i)) = x[i];
+  }
+}
+
+__global__ __launch_bounds__(256) void k_kv_read(KvParams p) {
+  __shared__ __attribute__((aligned(16))) uint8_t sC[KV_HEAD];
+  const uint32_t item = blockIdx.x, h = blockIdx.y;
+  const uint32_t b = kv_item_seq<KV_T>(p, item), base = kv_item_base<KV_T>(p, b);
+  const KvSeq s = kv_seq(p, b);
+  if (item < base || s.n == 0) return;
+  const uint32_t blk = s.pos / KV_T + (item - base);
+  if (blk * KV_T >= s.pos + s.n) return;
+  const int32_t held = p.len[b];
+  const uint32_t cap = p.max_pages * KV_T, len = !s.ok || held < 0 ? 0u : (uint32_t)held < cap ? (uint32_t)held : cap;
+  if (blockIdx.z == 0) read_block<0>(p, s, blk, len, h, sC);
+  else read_block<1>(p, s, blk, len, h, sC);
 }
 
 hipError_t launch_kv_append(const KvParams &p, hipStream_t s) {
