@@ -67,23 +67,39 @@ __device__ __forceinline__ KvSeq kv_seq(const KvParams &p, uint32_t b) {
   return s;
 }
 // Work items over a ragged batch: sequence b owns items f(b) .. f(b + 1) - 1 with f(b) = cu[b] / U + 2 b, at least as many as
-// the units of U rows or tokens that its rows touch, whatever its position; the last are idle. The sequence of an item: the largest b with f(b) <=
-// item, found by a 64-way search of one wave (a step for up to 64 sequences, two for 4096).
+// the blocks of U tokens that its rows touch, whatever its position; the last are idle. The sequence of an item is the
+// largest b with f(b) <= item: a 64-way search of one wave down to 64 sequences, of which lane i then reads all there is to
+// know about the i-th at once (one trip to memory for a batch of up to 64).
+struct KvItem { KvSeq s; uint32_t at; int32_t len; bool ok; };   // at: the item's place among the sequence's
 template <uint32_t U>
-__device__ __forceinline__ uint32_t kv_item_base(const KvParams &p, uint32_t b) { return kv_row0(p.cu, b, p.rows) / U + 2u * b; }
-template <uint32_t U>
-__device__ __forceinline__ uint32_t kv_item_seq(const KvParams &p, uint32_t item) {
+__device__ __forceinline__ KvItem kv_item(const KvParams &p, uint32_t item) {
   const uint32_t lane = threadIdx.x & 63u;
+  auto base = [&](uint32_t b) { return kv_row0(p.cu, b, p.rows) / U + 2u * b; };
   uint32_t lo = 0, n = p.B;
-  while (n > 1) {
+  while (n > 64) {
     const uint32_t step = (n + 63u) / 64u, off = lane * step;
-    const bool le = off < n && kv_item_base<U>(p, lo + off) <= item;
-    const uint64_t m = __ballot(le);
+    const uint64_t m = __ballot(off < n && base(lo + off) <= item);
     const uint32_t k = m ? 63u - (uint32_t)__builtin_clzll(m) : 0u;
     lo += k * step;
     n = n - k * step < step ? n - k * step : step;
   }
-  return __builtin_amdgcn_readfirstlane(lo);
+  const uint32_t b = lo + (lane < n ? lane : n - 1u);
+  const KvSeq s = kv_seq(p, b);
+  const int32_t len = p.len ? p.len[b] : 0;
+  const uint32_t f = s.r0 / U + 2u * b;
+  const uint64_t m = __ballot(lane < n && f <= item);
+  const uint32_t k = m ? 63u - (uint32_t)__builtin_clzll(m) : 0u;
+  KvItem o;
+  o.s.r0 = __builtin_amdgcn_readlane(s.r0, k);
+  o.s.n = __builtin_amdgcn_readlane(s.n, k);
+  o.s.pos = __builtin_amdgcn_readlane(s.pos, k);
+  o.s.slot = __builtin_amdgcn_readlane(s.slot, k);
+  o.s.ok = __builtin_amdgcn_readlane((uint32_t)s.ok, k) != 0;
+  o.len = (int32_t)__builtin_amdgcn_readlane((uint32_t)len, k);
+  const uint32_t fb = __builtin_amdgcn_readlane(f, k);
+  o.ok = m != 0;
+  o.at = item - fb;
+  return o;
 }
 // byte of key / value (token t of the block, d) in a head's 8 KB of codes
 __device__ __forceinline__ uint32_t kv_kcode(uint32_t t, uint32_t d) {

@@ -15,15 +15,60 @@ __device__ __forceinline__ uint16_t kv_finite(uint16_t x) {
   const uint16_t m = x & 0x7fffu;
   return m > 0x7c00u ? (uint16_t)0 : m == 0x7c00u ? (uint16_t)(x - 1) : x;
 }
-// x / s rounded to the nearest integer, ties to even, exactly: the estimate is off by less than one, and x - c s is exact
-// in one fma where it is near s / 2 (x has 11 bits and is at least s / 2 there; the difference needs no more than 24)
-__device__ __forceinline__ int kv_code(float x, float s, float rs) {
-  float c = __builtin_rintf(x * rs);
-  const float r = fmaf(-c, s, x), h = 0.5f * s;
-  const bool odd = ((int)c & 1) != 0;
-  if (r > h || (r == h && odd)) c += 1.0f;
-  else if (r < -h || (r == -h && odd)) c -= 1.0f;
-  return (int)c;
+// the low bytes of four words
+__device__ __forceinline__ uint32_t kv_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return perm(perm(d, c, 0x0c0c0400u), perm(b, a, 0x0c0c0400u), 0x05040100u);
+}
+// The bytes (code + 128) of a thread's 32 values, eight words of four: of consecutive d (keys) or of the four tokens of a d
+// (values). x / s is estimated as x rs, off by less than 2^-15, and the sum with 2^23 + 128 rounds it to the nearest integer.
+// Where an estimate of the wave lies within that of a border, all of them are settled exactly: x - c s takes no rounding where
+// it is near s / 2 (x has 11 bits and is at least s / 2 there, the difference needs no more than 24), and ties go to the even
+// code.
+template <int KV>
+__device__ __forceinline__ void kv_codes(const u16x8 *x, float s, uint32_t *w) {
+  const float rs = 1.0f / s, big = 8388608.0f + 128.0f;
+  auto val = [&](int g, int j) { return h_val(KV ? x[j][g] : x[g >> 1][4 * (g & 1) + j]); };
+  float far = 0.0f;
+#pragma unroll
+  for (int g = 0; g < 8; g++) {
+    float z[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float y = val(g, j) * rs;
+      z[j] = y + big;
+      far = fmaxf(far, fabsf(y - (z[j] - big)));
+    }
+    w[g] = kv_bytes(__float_as_uint(z[0]), __float_as_uint(z[1]), __float_as_uint(z[2]), __float_as_uint(z[3]));
+  }
+  if (__any(far > 0.5f - 0x1p-15f)) {
+    const float h = 0.5f * s;
+#pragma unroll
+    for (int g = 0; g < 8; g++) {
+      uint32_t z[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int c = (int)((w[g] >> (8 * j)) & 255u) - 128;
+        const float r = fmaf(-(float)c, s, val(g, j));
+        const bool odd = (c & 1) != 0;
+        z[j] = (uint32_t)(c + 128 + (r > h || (r == h && odd) ? 1 : r < -h || (r == -h && odd) ? -1 : 0));
+      }
+      w[g] = kv_bytes(z[0], z[1], z[2], z[3]);
+    }
+  }
+}
+// the largest |x| of a thread's values, as f16 bits (finite numbers order as integers; above: infinities, NaN)
+__device__ __forceinline__ uint32_t kv_amax(const u16x8 *x) {
+  const u16x8 m = {0x7fff, 0x7fff, 0x7fff, 0x7fff, 0x7fff, 0x7fff, 0x7fff, 0x7fff};
+  const u16x8 a = __builtin_elementwise_max(__builtin_elementwise_max(x[0] & m, x[1] & m), __builtin_elementwise_max(x[2] & m, x[3] & m));
+  uint32_t r = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) r = max(r, (uint32_t)a[j]);
+  return r;
+}
+__device__ __forceinline__ void kv_hold(u16x8 *x) {       // infinities to the largest value, NaN to 0
+  if (kv_amax(x) < 0x7c00u) return;
+#pragma unroll
+  for (int i = 0; i < 32; i++) x[i >> 3][i & 7] = kv_finite(x[i >> 3][i & 7]);
 }
 
 // One workgroup takes one block of one sequence and kv head, keys or values, and every thread 32 of its values, in
@@ -35,22 +80,27 @@ struct Part {
   uint32_t tid;
   __device__ uint32_t tok(int i) const { return KV ? 4 * (tid >> 4) + i : tid >> 2; }                               // token and
   __device__ uint32_t d(int i) const { return KV ? 8 * (tid & 15) : 16 * (tid & 3) + (i >> 1) * 64 + (i & 1) * 8; }   // first d of x[i]
-  // x from / to the tail, the values whose token passes `is`
+  // x from / to the tail, the values whose token passes `is` (load: by the whole workgroup; a piece of values holds eight
+  // tokens of a d, so they go through LDS, 16 KB as [four tokens][d])
   template <class F>
-  __device__ void load_tail(const uint16_t *tail, u16x8 *x, F is) const {
+  __device__ void load_tail(const uint16_t *tail, u16x8 *x, uint8_t *lds, F is) const {
     if constexpr (KV == 0) {
       if (is(tok(0))) {
 #pragma unroll
         for (int i = 0; i < 4; i++) x[i] = *(const u16x8 *)(tail + kv_ktail(tok(0), d(i)));
       }
     } else {
-      bool any = false;
 #pragma unroll
-      for (int i = 0; i < 4; i++) any |= is(tok(i));
-      if (!any) return;
+      for (int i = 0; i < 4; i++) {
+        const uint32_t pc = tid + 256 * i, g = 8 * (pc >> 9) + ((pc >> 4) & 3), dd = 16 * ((pc >> 6) & 7) + (pc & 15);
+        const u32x4 w = *(const u32x4 *)(tail + 8 * pc);
+        *(u32x2 *)(lds + (g * KV_D + dd) * 8) = (u32x2){w.x, w.y};
+        *(u32x2 *)(lds + ((g + 4) * KV_D + dd) * 8) = (u32x2){w.z, w.w};
+      }
+      __syncthreads();
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const u16x4 w = *(const u16x4 *)(tail + kv_vtail(tok(0), d(0) + j));
+        const u16x4 w = *(const u16x4 *)(lds + ((tid >> 4) * KV_D + d(0) + j) * 8);
 #pragma unroll
         for (int i = 0; i < 4; i++)
           if (is(tok(i))) x[i][j] = w[i];
@@ -90,18 +140,16 @@ __device__ void append_block(const KvParams &p, const KvSeq &s, uint32_t blk, ui
   const Part<KV> part{tid};
   const uint16_t *X = (KV ? p.V : p.K) + (KV ? p.vhs : p.khs) * h;
   const uint64_t rs = KV ? p.vrs : p.krs;
+  const uint32_t page = kv_page(p, s.slot, blk);
   u16x8 x[4];
   // the values of a block that this call brings
   auto fresh = [&](uint32_t block) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const uint32_t t = block * KV_T + part.tok(i);
-      if (t >= s.pos && t < end) {
-        x[i] = *(const u16x8 *)(X + rs * (s.r0 + (t - s.pos)) + part.d(i));
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[i][j] = kv_finite(x[i][j]);
-      }
+      if (t >= s.pos && t < end) x[i] = *(const u16x8 *)(X + rs * (s.r0 + (t - s.pos)) + part.d(i));
     }
+    kv_hold(x);
   };
   auto keep = [&](uint32_t block) {              // and into the tail
     part.store_tail(p.tail + kv_tail_at(p, s.slot, block, h, KV), x, [&](uint32_t t) {
@@ -118,42 +166,26 @@ __device__ void append_block(const KvParams &p, const KvSeq &s, uint32_t blk, ui
   if (blk + 1 >= last && (blk == k0 || ((blk ^ k0) & 1))) keep(blk);
   if ((blk + 1) * KV_T <= end) {
     if (blk * KV_T < s.pos) {
-      part.load_tail(p.tail + kv_tail_at(p, s.slot, blk, h, KV), x, [&](uint32_t t) { return blk * KV_T + t < s.pos; });
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[i][j] = kv_finite(x[i][j]);   // (a tail that no call has written)
+      part.load_tail(p.tail + kv_tail_at(p, s.slot, blk, h, KV), x, sC, [&](uint32_t t) { return blk * KV_T + t < s.pos; });
+      kv_hold(x);                                // (a tail that no call has written)
     }
-    uint32_t mx = 0;                             // |x| as bits: finite f16 order as integers
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) mx = max(mx, (uint32_t)(x[i][j] & 0x7fffu));
+    uint32_t mx = kv_amax(x);
     for (int o = 32; o; o >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
     if ((tid & 63) == 0) sMax[tid >> 6] = h_val((uint16_t)mx);
     __syncthreads();
     const float amax = fmaxf(fmaxf(sMax[0], sMax[1]), fmaxf(sMax[2], sMax[3]));
-    const float sc = amax > 0.0f ? amax / 127.0f : 1.0f, ri = 1.0f / sc;
-    const uint32_t page = kv_page(p, s.slot, blk);
+    const float sc = amax > 0.0f ? amax / 127.0f : 1.0f;
     const bool have = page != 0xffffffffu;
     uint8_t *codes = p.codes + kv_code_at(p, have ? page : 0u, h, KV);
-    auto code = [&](uint16_t v) { return (uint32_t)(kv_code(h_val(v), sc, ri) + 128); };
+    uint32_t w[8];
+    kv_codes<KV>(x, sc, w);
     if constexpr (KV == 0) {
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        u32x4 w;
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-          const u16x8 &v = x[2 * i + (g >> 1)];
-          const int j = 4 * (g & 1);
-          w[g] = code(v[j]) | code(v[j + 1]) << 8 | code(v[j + 2]) << 16 | code(v[j + 3]) << 24;
-        }
-        if (have) *(u32x4 *)(codes + kv_kcode(part.tok(0), part.d(2 * i))) = w;
-      }
+      for (int i = 0; i < 2; i++)
+        if (have) *(u32x4 *)(codes + kv_kcode(part.tok(0), part.d(2 * i))) = (u32x4){w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        *(uint32_t *)(sC + kv_vcode(part.tok(0), part.d(0) + j)) = code(x[0][j]) | code(x[1][j]) << 8 | code(x[2][j]) << 16 | code(x[3][j]) << 24;
+      for (int j = 0; j < 8; j++) *(uint32_t *)(sC + kv_vcode(part.tok(0), part.d(0) + j)) = w[j];
       __syncthreads();
       if (have) {
 #pragma unroll
@@ -172,14 +204,14 @@ __device__ void append_block(const KvParams &p, const KvSeq &s, uint32_t blk, ui
   }
 }
 
-__global__ __launch_bounds__(256) void k_kv_append(KvParams p) {
-  __shared__ __attribute__((aligned(16))) uint8_t sC[KV_HEAD];
+__global__ __launch_bounds__(256, 8) void k_kv_append(KvParams p) {
+  __shared__ __attribute__((aligned(16))) uint8_t sC[2 * KV_HEAD];
   __shared__ float sMax[4];
-  const uint32_t item = blockIdx.x, h = blockIdx.y;
-  const uint32_t b = kv_item_seq<KV_T>(p, item), base = kv_item_base<KV_T>(p, b);
-  const KvSeq s = kv_seq(p, b);
-  if (item < base || !s.ok || s.n == 0) return;
-  const uint32_t cap = p.max_pages * KV_T, k0 = s.pos / KV_T, blk = k0 + (item - base);
+  const uint32_t h = blockIdx.y;
+  const KvItem it = kv_item<KV_T>(p, blockIdx.x);
+  const KvSeq &s = it.s;
+  if (!it.ok || !s.ok || s.n == 0) return;
+  const uint32_t cap = p.max_pages * KV_T, k0 = s.pos / KV_T, blk = k0 + it.at;
   const uint32_t end = s.pos + s.n < cap ? s.pos + s.n : cap;
   if (blk >= p.max_pages || blk * KV_T >= end) return;
   if (blockIdx.z == 0) append_block<0>(p, s, blk, k0, end, h, sC, sMax);
@@ -202,7 +234,7 @@ __device__ void read_block(const KvParams &p, const KvSeq &s, uint32_t blk, uint
   for (int i = 0; i < 4; i++) x[i] = (u16x8){};
   const uint32_t page = blk < len / KV_T ? kv_page(p, s.slot, blk) : 0xffffffffu;
   if (blk == len / KV_T) {
-    part.load_tail(p.tail + kv_tail_at(p, s.slot, blk, h, KV), x, [&](uint32_t t) { return blk * KV_T + t < len; });
+    part.load_tail(p.tail + kv_tail_at(p, s.slot, blk, h, KV), x, sC, [&](uint32_t t) { return blk * KV_T + t < len; });
   } else if (page != 0xffffffffu) {
     const uint8_t *codes = p.codes + kv_code_at(p, page, h, KV);
     const float sc = p.scales[kv_scale_at(p, page, h, KV)];
@@ -234,14 +266,14 @@ __device__ void read_block(const KvParams &p, const KvSeq &s, uint32_t blk, uint
 }
 
 __global__ __launch_bounds__(256) void k_kv_read(KvParams p) {
-  __shared__ __attribute__((aligned(16))) uint8_t sC[KV_HEAD];
-  const uint32_t item = blockIdx.x, h = blockIdx.y;
-  const uint32_t b = kv_item_seq<KV_T>(p, item), base = kv_item_base<KV_T>(p, b);
-  const KvSeq s = kv_seq(p, b);
-  if (item < base || s.n == 0) return;
-  const uint32_t blk = s.pos / KV_T + (item - base);
+  __shared__ __attribute__((aligned(16))) uint8_t sC[2 * KV_HEAD];
+  const uint32_t h = blockIdx.y;
+  const KvItem it = kv_item<KV_T>(p, blockIdx.x);
+  const KvSeq &s = it.s;
+  if (!it.ok || s.n == 0) return;
+  const uint32_t blk = s.pos / KV_T + it.at;
   if (blk * KV_T >= s.pos + s.n) return;
-  const int32_t held = p.len[b];
+  const int32_t held = it.len;
   const uint32_t cap = p.max_pages * KV_T, len = !s.ok || held < 0 ? 0u : (uint32_t)held < cap ? (uint32_t)held : cap;
   if (blockIdx.z == 0) read_block<0>(p, s, blk, len, h, sC);
   else read_block<1>(p, s, blk, len, h, sC);
