@@ -152,7 +152,12 @@ unsigned kv_attention_counters(int cus);
 hipError_t launch_rope(const RopeParams &p, hipStream_t s);
 hipError_t launch_kv_append(const KvParams &p, hipStream_t s);
 hipError_t launch_kv_read(const KvParams &p, hipStream_t s);
-// ws: part / cnt may be used
-hipError_t launch_kv_attention(const KvParams &p, int cus, bool ws, float *part, unsigned *cnt, hipStream_t s);
+// with many queries: runs into which a block's keys are divided where the blocks alone do not fill the GPU (0, 1: none), and
+// the bytes that a run leaves
+unsigned kv_attention_runs(const KvParams &p, int cus);
+uint64_t kv_attention_run_bytes(const KvParams &p);
+// ws: part / cnt may be used; S > 1: rpart holds S runs
+hipError_t launch_kv_attention(const KvParams &p, int cus, bool ws, float *part, unsigned *cnt, unsigned S, float *rpart,
+                               hipStream_t s);
 
 }  // namespace p0k

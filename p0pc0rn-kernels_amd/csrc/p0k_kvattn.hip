@@ -18,6 +18,26 @@ __device__ __forceinline__ uint32_t pack_o(float a, float b) {
   return pack2(a, b);
 }
 
+// z -> tanh(z). Up to |z| = 0.75 (scores up to 3/4 of the cap: nearly all) by an odd polynomial, fitted here for the least
+// largest error (1.9e-7) on that range: 6 operations at full rate, where the exponential and the reciprocal of the other form
+// take a quarter of it (two chunks of 1145 queries after 12000 tokens, cap 30: CAPT)
+template <int N>
+__device__ __forceinline__ void soft_cap(float (&z)[N]) {
+  float mx = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; i++) mx = fmaxf(mx, fabsf(z[i]));
+  if (__any(!(mx <= 0.75f))) {
+#pragma unroll
+    for (int i = 0; i < N; i++) z[i] = 2.0f * sigmoid(2.0f * z[i]) - 1.0f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const float u = z[i] * z[i];
+      z[i] *= fmaf(u, fmaf(u, fmaf(u, fmaf(u, 0.012318825796f, -0.049280440068f), 0.132260913444f), -0.33323076443f), 0.999997228305f);
+    }
+  }
+}
+
 // What a sequence asks of the kernel: units of 32 tokens, those of the sinks [0, su) and then from unit `lo` on (0 units:
 // nothing to do; a sequence that sees nothing has one that is all masked, for its rows have to be written)
 struct KvWork { KvSeq s; uint32_t end, su, lo, units, blocks, io; };   // io: the first unit of the open block, by its place
@@ -230,7 +250,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_kv_attn_split(KvParams p, u
     }
     clear();
     float svc = 1.0f;                                                             // what O is held in units of
-    const float sl2 = CAP ? p.scale : p.scale * 1.4426950408889634f;
+    const float sl2 = CAP ? p.scale / p.cap : p.scale * 1.4426950408889634f;
 
     auto unit_of = [&](uint32_t i) { return i < w.su ? i : i - w.su + w.lo; };
     // one unit: scores, softmax, products. kf(tt, s), vf(d): the A operands; then(): once the keys are used
@@ -256,9 +276,11 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_kv_attn_split(KvParams p, u
       for (int nb = 0; nb < NB; nb++) {
         float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          x[i] = s[nb][i >> 2][i & 3] * f;
-          if constexpr (CAP) x[i] = p.cap * 1.4426950408889634f * (2.0f * sigmoid(2.0f * x[i] / p.cap) - 1.0f);
+        for (int i = 0; i < 8; i++) x[i] = s[nb][i >> 2][i & 3] * f;
+        if constexpr (CAP) {
+          soft_cap(x);
+#pragma unroll
+          for (int i = 0; i < 8; i++) x[i] *= p.cap * 1.4426950408889634f;
         }
         if (none || __any(k0 + 32 > kmax[nb] || (k0 < wlo[nb] && k0 + 32 > p.sinks))) {
 #pragma unroll
@@ -472,13 +494,13 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_kv_attn_split(KvParams p, u
 // transposing read. The keys' scale multiplies the scores. The values' scale goes into the exponent: O is held in units of
 // `ref`, which moves (and O with it) only when a block's scale leaves [ref, 64 ref].
 template <int NW, bool CAP>
-__global__ __launch_bounds__(64 * NW, 2) void k_kv_attn_block(KvParams p, uint32_t items) {
+__global__ __launch_bounds__(64 * NW, 2) void k_kv_attn_block(KvParams p, uint32_t items, uint32_t S, float *part) {
   constexpr uint32_t RB = 32 * NW, NP = 512 / (64 * NW);                          // pieces of 16 codes a thread moves, keys and values each
   __shared__ __attribute__((aligned(16))) f16 sK[2][KV_HEAD], sV[2][KV_HEAD];     // [8 d][token], [32 tokens][group][d]: pieces of 8
   const uint32_t tid = threadIdx.x, lane = tid & 63, gh = lane >> 5, l32 = lane & 31, wave = rfl(tid >> 6);
   const uint32_t rep = p.Hq / p.Hkv;
   // kv heads go round the XCDs, so that a head's codes stay in one L2; the longest (last) blocks first
-  const uint32_t hk = blockIdx.x % p.Hkv, item = items - 1 - blockIdx.x / p.Hkv;
+  const uint32_t hk = blockIdx.x % p.Hkv, by = blockIdx.x / p.Hkv, item = items - 1 - by % items, run = by / items;
   auto base_of = [&](uint32_t b) { return (uint32_t)((uint64_t)kv_row0(p.cu, b, p.rows) * rep / RB) + b; };
   uint32_t b = 0;
   {
@@ -506,8 +528,11 @@ __global__ __launch_bounds__(64 * NW, 2) void k_kv_attn_block(KvParams p, uint32
     lo = l0 < all ? l0 : all;
     su = s0 < lo ? s0 : lo;
   }
-  const uint32_t nt = su + (all - lo);                                            // tiles: [0, su), [lo, all)
-  auto tile_of = [&](uint32_t i) { return i < su ? i : i - su + lo; };
+  // tiles: [0, su), [lo, all), of which this workgroup takes its run (of four at least; fewer runs than S then)
+  const uint32_t ntile = su + (all - lo), runs = S == 1 ? 1u : (ntile + 3) / 4 < S ? (ntile + 3) / 4 : S;
+  const uint32_t t0 = run < runs ? (uint32_t)((uint64_t)ntile * run / runs) : 0u;
+  const uint32_t nt = run < runs ? (uint32_t)((uint64_t)ntile * (run + 1) / runs) - t0 : 0u;
+  auto tile_of = [&](uint32_t i) { return t0 + i < su ? t0 + i : t0 + i - su + lo; };
 
   uint32_t row = row0 + wave * 32 + l32;
   const bool live = row < rows;
@@ -585,7 +610,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_kv_attn_block(KvParams p, uint32
 #pragma unroll
   for (int i = 0; i < 4; i++) oacc[i] = (f32x16){};
   float m = -1.0e30f, l = 0.0f, ref = 0.0f;                                       // ref 0: none yet
-  const float sl2 = CAP ? p.scale : p.scale * 1.4426950408889634f;
+  const float sl2 = CAP ? p.scale / p.cap : p.scale * 1.4426950408889634f;
   uint32_t gc = NONE;
   float sk = 1.0f, sv = 1.0f, skn = 1.0f, svn = 1.0f;
   if (nt) {
@@ -625,11 +650,13 @@ __global__ __launch_bounds__(64 * NW, 2) void k_kv_attn_block(KvParams p, uint32
     const uint32_t k0 = tile_of(i) * KV_T;
     float sf = f;
     if constexpr (CAP) {
+      float z[32];
 #pragma unroll
-      for (int kb = 0; kb < 2; kb++)
+      for (int r = 0; r < 32; r++) z[r] = sacc[r >> 4][r & 15] * f;
+      soft_cap(z);
 #pragma unroll
-        for (int r = 0; r < 16; r++) sacc[kb][r] = p.cap * (2.0f * sigmoid(2.0f * sacc[kb][r] * f / p.cap) - 1.0f);
-      sf = 1.4426950408889634f;
+      for (int r = 0; r < 32; r++) sacc[r >> 4][r & 15] = z[r];
+      sf = p.cap * 1.4426950408889634f;
     }
     if (gi == NONE || __any(k0 + KV_T > kmax || (k0 < wlo && k0 + KV_T > p.sinks))) {
 #pragma unroll
@@ -691,16 +718,57 @@ __global__ __launch_bounds__(64 * NW, 2) void k_kv_attn_block(KvParams p, uint32
   }
 
   const float lt = l + __shfl_xor(l, 32, 64);
-  const float inv = lt > 0.0f ? ref / lt : 0.0f;
-  if (live) {
-    u16 *o = p.Ko + (uint64_t)(s.r0 + qi) * p.ldo + h * KV_D + 4 * gh;
+  if (!live) return;
+  if (S > 1) {
+    // one of several runs: its part by (run, row, head), and what it is: the maximum and sum of the row; sum -1: not there.
+    // Where there is only one run after all, its rows are finished here (-2)
+    float *pr = part + ((uint64_t)run * p.rows * p.Hq + (uint64_t)(s.r0 + qi) * p.Hq + h) * (KV_D + 2);
+    if (gh == 0) *(f32x2 *)pr = (f32x2){m, run >= runs ? -1.0f : runs <= 1 ? -2.0f : lt};
+    if (run >= runs && run) return;
+    if (runs > 1) {
 #pragma unroll
-    for (int db = 0; db < 4; db++)
+      for (int db = 0; db < 4; db++)
 #pragma unroll
-      for (int g4 = 0; g4 < 4; g4++)
-        *(u32x2 *)(o + 32 * db + 8 * g4) = (u32x2){pack_o(oacc[db][4 * g4] * inv, oacc[db][4 * g4 + 1] * inv),
-                                                  pack_o(oacc[db][4 * g4 + 2] * inv, oacc[db][4 * g4 + 3] * inv)};
+        for (int g4 = 0; g4 < 4; g4++) {
+          float *o = pr + 2 + 32 * db + 8 * g4 + 4 * gh;
+          *(f32x2 *)o = (f32x2){oacc[db][4 * g4] * ref, oacc[db][4 * g4 + 1] * ref};
+          *(f32x2 *)(o + 2) = (f32x2){oacc[db][4 * g4 + 2] * ref, oacc[db][4 * g4 + 3] * ref};
+        }
+      return;
+    }
   }
+  const float inv = lt > 0.0f ? ref / lt : 0.0f;
+  u16 *o = p.Ko + (uint64_t)(s.r0 + qi) * p.ldo + h * KV_D + 4 * gh;
+#pragma unroll
+  for (int db = 0; db < 4; db++)
+#pragma unroll
+    for (int g4 = 0; g4 < 4; g4++)
+      *(u32x2 *)(o + 32 * db + 8 * g4) = (u32x2){pack_o(oacc[db][4 * g4] * inv, oacc[db][4 * g4 + 1] * inv),
+                                                pack_o(oacc[db][4 * g4 + 2] * inv, oacc[db][4 * g4 + 3] * inv)};
+}
+
+// The runs of k_kv_attn_block together: a half wave for a row of a head, four d a thread
+__global__ __launch_bounds__(256) void k_kv_attn_join(KvParams p, uint32_t S, const float *part) {
+  const uint64_t it = (uint64_t)blockIdx.x * 256 + threadIdx.x, rh = it >> 5, n = (uint64_t)p.rows * p.Hq;
+  if (rh >= n) return;
+  const uint32_t r = (uint32_t)(rh / p.Hq), h = (uint32_t)(rh - (uint64_t)r * p.Hq), d = 4 * ((uint32_t)it & 31u);
+  if (r < kv_row0(p.cu, 0, p.rows) || r >= kv_row0(p.cu, p.B, p.rows)) return;
+  const float *pr = part + rh * (KV_D + 2);
+  const uint64_t step = n * (KV_D + 2);
+  float M = -1.0e30f, L = 0.0f;
+  f32x4 o = (f32x4){};
+  for (uint32_t i = 0; i < S; i++, pr += step) {
+    const f32x2 ml = *(const f32x2 *)pr;
+    if (ml.y == -2.0f) return;
+    if (ml.y == -1.0f) break;
+    const f32x2 a = *(const f32x2 *)(pr + 2 + d), b = *(const f32x2 *)(pr + 4 + d);
+    const float mn = fmaxf(M, ml.x), f1 = __builtin_amdgcn_exp2f(M - mn), f2 = __builtin_amdgcn_exp2f(ml.x - mn);
+    o = o * f1 + (f32x4){a.x, a.y, b.x, b.y} * f2;
+    L = L * f1 + ml.y * f2;
+    M = mn;
+  }
+  const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+  *(u32x2 *)(p.Ko + (uint64_t)r * p.ldo + h * KV_D + d) = (u32x2){pack_o(o.x * inv, o.y * inv), pack_o(o.z * inv, o.w * inv)};
 }
 
 uint64_t kv_attention_part_bytes(int cus) {
@@ -708,14 +776,31 @@ uint64_t kv_attention_part_bytes(int cus) {
 }
 unsigned kv_attention_counters(int cus) { return (unsigned)cus; }
 
-hipError_t launch_kv_attention(const KvParams &p, int cus, bool ws, float *part, unsigned *cnt, hipStream_t s) {
+// rows of one kv head of a sequence, on average: which kernel takes the call
+static uint64_t rows_per_seq(const KvParams &p) { return ((uint64_t)p.rows * (p.Hq / p.Hkv) + p.B - 1) / p.B; }
+constexpr uint32_t KVA_BLOCK = 256;               // rows of a block of k_kv_attn_block
+static uint32_t block_items(const KvParams &p) { return (uint32_t)((uint64_t)p.rows * (p.Hq / p.Hkv) / KVA_BLOCK + p.B); }
+
+unsigned kv_attention_runs(const KvParams &p, int cus) {
+  const char *e = getenv("KVT_S");
+  if (rows_per_seq(p) <= 64 || p.max_pages < 8) return 0;
+  const uint64_t groups = (uint64_t)block_items(p) * p.Hkv;
+  return groups >= 2u * cus ? 1u : std::max(1u, std::min(e ? atoi(e) : 8u, (unsigned)((2u * cus + groups - 1) / groups)));
+}
+uint64_t kv_attention_run_bytes(const KvParams &p) { return (uint64_t)p.rows * p.Hq * (KV_D + 2) * sizeof(float); }
+
+hipError_t launch_kv_attention(const KvParams &p, int cus, bool ws, float *part, unsigned *cnt, unsigned S, float *rpart, hipStream_t s) {
   if (p.rows == 0 || p.B == 0 || p.Hq == 0) return hipSuccess;
-  const uint64_t rows = (uint64_t)p.rows * (p.Hq / p.Hkv), per = (rows + p.B - 1) / p.B;
+  const uint64_t per = rows_per_seq(p);
   if (per > 64) {
-    const uint32_t items = (uint32_t)(rows / 256 + p.B);
-    const dim3 grid(items * p.Hkv), block(512);
-    if (p.cap > 0.0f) hipLaunchKernelGGL((k_kv_attn_block<8, true>), grid, block, 0, s, p, items);
-    else hipLaunchKernelGGL((k_kv_attn_block<8, false>), grid, block, 0, s, p, items);
+    const uint32_t items = block_items(p);
+    const dim3 grid(items * p.Hkv * S), block(512);
+    if (p.cap > 0.0f) hipLaunchKernelGGL((k_kv_attn_block<8, true>), grid, block, 0, s, p, items, S, rpart);
+    else hipLaunchKernelGGL((k_kv_attn_block<8, false>), grid, block, 0, s, p, items, S, rpart);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || S == 1) return e;
+    const uint64_t threads = (uint64_t)p.rows * p.Hq * 32;
+    hipLaunchKernelGGL(k_kv_attn_join, dim3((uint32_t)((threads + 255) / 256)), dim3(256), 0, s, p, S, rpart);
     return hipGetLastError();
   }
   auto go = [&](auto kernel, int nw) { hipLaunchKernelGGL(kernel, dim3(cus), dim3(64 * nw), 0, s, p, ws ? 1u : 0u, part, cnt); };

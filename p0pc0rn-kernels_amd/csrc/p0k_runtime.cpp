@@ -1002,7 +1002,18 @@ int p0k_kv_attention(p0k_ctx *c, const p0k_kv_attn_args *a) {
   if (int rr = ws_allowed(c, &capturing, &ws)) return rr;
   if (ws) c->capture_ws = true;
   const int cus = [&] { std::lock_guard<std::mutex> lk(c->mu); return (int)c->tune.cus; }();
-  hipError_t e = p0k::launch_kv_attention(p, cus, ws, c->ws_kv, c->ws_kv_cnt, c->stream);
+  unsigned S = std::max(1u, p0k::kv_attention_runs(p, cus));
+  float *rpart = nullptr;
+  if (S > 1) {
+    // (no workspace to be had: one run)
+    if (int rr = WsSource{c, nullptr}.slices_if(0, S * p0k::kv_attention_run_bytes(p), &rpart)) return rr;
+    if (!rpart) S = 1;
+    if (capturing) {
+      std::lock_guard<std::mutex> lk(c->mu);
+      c->graph_epoch++;                  // (the graph may hold the workspace)
+    }
+  }
+  hipError_t e = p0k::launch_kv_attention(p, cus, ws, c->ws_kv, c->ws_kv_cnt, S, rpart, c->stream);
   if (e != hipSuccess) return hip_err(e, "kv_attention launch");
   return P0K_OK;
 }
