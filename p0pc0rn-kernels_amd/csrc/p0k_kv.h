@@ -152,7 +152,7 @@ unsigned kv_attention_counters(int cus);
 hipError_t launch_rope(const RopeParams &p, hipStream_t s);
 hipError_t launch_kv_append(const KvParams &p, hipStream_t s);
 hipError_t launch_kv_read(const KvParams &p, hipStream_t s);
-// with many queries: runs into which a block's keys are divided where the blocks alone do not fill the GPU (0, 1: none), and
+// with many queries: runs into which a block's keys are divided where the blocks alone do not fill the GPU (1: not at all), and
 // the bytes that a run leaves
 unsigned kv_attention_runs(const KvParams &p, int cus);
 uint64_t kv_attention_run_bytes(const KvParams &p);

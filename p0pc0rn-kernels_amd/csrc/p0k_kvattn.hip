@@ -20,7 +20,7 @@ __device__ __forceinline__ uint32_t pack_o(float a, float b) {
 
 // z -> tanh(z). Up to |z| = 0.75 (scores up to 3/4 of the cap: nearly all) by an odd polynomial, fitted here for the least
 // largest error (1.9e-7) on that range: 6 operations at full rate, where the exponential and the reciprocal of the other form
-// take a quarter of it (two chunks of 1145 queries after 12000 tokens, cap 30: CAPT)
+// take a quarter of it (two chunks of 1145 queries after 12000 tokens, cap 30: 818 us with that form, 456 with this)
 template <int N>
 __device__ __forceinline__ void soft_cap(float (&z)[N]) {
   float mx = 0.0f;
@@ -90,12 +90,22 @@ __device__ __forceinline__ float rlf(float v, uint32_t l) { return __uint_as_flo
 // A lane owns a query (of the 16 columns of a 16x16x32 product) as in S^T = K Q^T, O^T += V^T P: the scores that it holds are
 // the B operand of the second product, and the cache's layout makes 16-byte loads the A operands of both. Codes are exact
 // in f16; the scales stay in fp32: the keys' multiplies the scores, and O is held in units of the current block's value scale.
-template <int NB, int NW, bool CAP>
-__global__ __launch_bounds__(64 * NW, NW / 4) void k_kv_attn_split(KvParams p, uint32_t ws, float *part, uint32_t *cnt) {
+//
+// NB: blocks of 16 or 32 rows. 16 read the keys of 17 and more rows twice and more, but start and end sooner; the result is
+// false (and nothing done) where 32 are the better choice, see k_kv_attn_split.
+constexpr int KVA_NW = 8;                         // waves of a workgroup
+struct KvaShared {
+  __attribute__((aligned(16))) float o[KVA_NW][2 * 8 * 64 * 4];                   // parts of groups that waves share
+  float m[KVA_NW][2 * 64], l[KVA_NW][2 * 64];
+  uint32_t job[2][7];                                                             // groups whose last part this workgroup brought
+};
+template <int NB, bool CAP>
+__device__ __forceinline__ bool attn_split(const KvParams &p, uint32_t ws, float *part, uint32_t *cnt, KvaShared &sh_) {
+  constexpr int NW = KVA_NW;
   constexpr uint32_t RB = 16 * NB, PART = kva_part(RB);
-  __shared__ __attribute__((aligned(16))) float sO[NW][NB * 8 * 64 * 4];
-  __shared__ float sM[NW][NB * 64], sL[NW][NB * 64];
-  __shared__ uint32_t sJob[2][7];                                                 // groups whose last part this workgroup brought
+  auto &sO = sh_.o;
+  auto &sM = sh_.m, &sL = sh_.l;
+  auto &sJob = sh_.job;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = rfl(tid >> 6), r16 = lane & 15, q4 = lane >> 4;
   const uint32_t rep = p.Hq / p.Hkv;
   if (tid < 2) sJob[tid][0] = 0;
@@ -140,11 +150,26 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_kv_attn_split(KvParams p, u
     *base = at + (f ? __builtin_amdgcn_readlane(sum, f - 1) : 0u);
     return cb + f;
   };
+  if constexpr (NB == 1) {
+    // more than 64 units a workgroup, and a quarter less of them with blocks of 32 rows
+    if (T > 64 * gridDim.x) {
+      uint32_t T2 = 0;
+      for (uint32_t b0 = 0; b0 < p.B; b0 += 64) {
+        uint32_t t = 0;
+        if (b0 + lane < p.B) {
+          const KvWork w = kv_work<2 * RB>(p, b0 == cb ? ls : kv_seq(p, b0 + lane));
+          t = w.units * w.blocks * p.Hkv;
+        }
+        T2 += __builtin_amdgcn_readlane(wave_scan(t), 63);
+      }
+      if (T2 <= T - T / 4) return false;
+    }
+  }
   uint32_t nwg = (T + 3) / 4;                                                     // at least 4 units each
   nwg = nwg < gridDim.x ? nwg : gridDim.x;
   // (row blocks that share their keys go to one XCD)
   const uint32_t blk = blockIdx.x, k = NB > 1 && nwg == gridDim.x && (nwg & 7u) == 0u ? (blk & 7u) * (nwg >> 3) + (blk >> 3) : blk;
-  if (k >= nwg) return;
+  if (k >= nwg) return true;
   const uint32_t uq = T / nwg, ur = T - uq * nwg;
   auto first = [&](uint32_t i) { return uq * i + (i < ur ? i : ur); };            // the first unit of workgroup i
   auto owner = [&](uint32_t u) { return u < ur * (uq + 1) ? u / (uq + 1) : ur + (u - ur * (uq + 1)) / uq; };
@@ -159,7 +184,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_kv_attn_split(KvParams p, u
       }
       (i ? we : wa) = rfl(u);
     }
-    if (wa >= we) return;
+    if (wa >= we) return true;
   }
   const uint32_t per = (we - wa + NW - 1) / NW;
   auto wfirst = [&](uint32_t i) { const uint32_t u = wa + i * per; return u < we ? u : we; };
@@ -484,6 +509,16 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_kv_attn_split(KvParams p, u
     }
     if (tid == 0) __hip_atomic_store(cnt + kf, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
   }
+  return true;
+}
+
+// Which blocks: measured over 2 head layouts, batches of 1 and 8, 1000 and 8000 keys and 8 to 256 rows, the two cross where
+// blocks of 16 rows come to about 64 units a CU (24 rows, 64 heads of 8000 keys: 51.6 us against 34.8 with 32; 8 heads: 15.9
+// against 22.3); up to 16 rows, 32 only add work. The lengths are known here, not on the host.
+template <bool CAP>
+__global__ __launch_bounds__(64 * KVA_NW, 2) void k_kv_attn_split(KvParams p, uint32_t ws, float *part, uint32_t *cnt) {
+  __shared__ KvaShared sh;
+  if (!attn_split<1, CAP>(p, ws, part, cnt, sh)) attn_split<2, CAP>(p, ws, part, cnt, sh);
 }
 
 // ---------------------------------------------------------------------------------------- many queries
@@ -772,27 +807,32 @@ __global__ __launch_bounds__(256) void k_kv_attn_join(KvParams p, uint32_t S, co
 }
 
 uint64_t kv_attention_part_bytes(int cus) {
-  return (uint64_t)cus * 2 * kva_part(64) * sizeof(float);
+  return (uint64_t)cus * 2 * kva_part(32) * sizeof(float);
 }
 unsigned kv_attention_counters(int cus) { return (unsigned)cus; }
 
-// rows of one kv head of a sequence, on average: which kernel takes the call
-static uint64_t rows_per_seq(const KvParams &p) { return ((uint64_t)p.rows * (p.Hq / p.Hkv) + p.B - 1) / p.B; }
+// Which kernel: blocks of 256 rows where a sequence and kv head have more than that on average and all rows of all heads are
+// more than 20 a CU; runs of keys otherwise. Measured over 2 head layouts, batches of 1 and 8, 1000 and 8000 keys, 16 to 1024
+// rows: 8 heads x 512 rows, 8000 keys: runs 46.5 us, blocks 50.6; x 768: 60.2 and 52.7; 64 heads x 256 rows: 140 and 142 (1000
+// keys: 25.7 and 45.6); x 384: 210 and 157 (37 and 51)
+static bool by_blocks(const KvParams &p, int cus) {
+  return (uint64_t)p.rows * (p.Hq / p.Hkv) > 256ull * p.B && (uint64_t)p.rows * p.Hq > 20ull * cus;
+}
 constexpr uint32_t KVA_BLOCK = 256;               // rows of a block of k_kv_attn_block
 static uint32_t block_items(const KvParams &p) { return (uint32_t)((uint64_t)p.rows * (p.Hq / p.Hkv) / KVA_BLOCK + p.B); }
 
+// Runs of a block's keys: two workgroups for each CU between all blocks, eight at most (two chunks of 1145 queries after 12000
+// keys, 152 blocks: one run 456 us, two 349, three 327, four 315)
 unsigned kv_attention_runs(const KvParams &p, int cus) {
-  const char *e = getenv("KVT_S");
-  if (rows_per_seq(p) <= 64 || p.max_pages < 8) return 0;
+  if (!by_blocks(p, cus) || p.max_pages < 8) return 1;
   const uint64_t groups = (uint64_t)block_items(p) * p.Hkv;
-  return groups >= 2u * cus ? 1u : std::max(1u, std::min(e ? atoi(e) : 8u, (unsigned)((2u * cus + groups - 1) / groups)));
+  return groups >= 2u * cus ? 1u : std::min(8u, (unsigned)((2u * cus + groups - 1) / groups));
 }
 uint64_t kv_attention_run_bytes(const KvParams &p) { return (uint64_t)p.rows * p.Hq * (KV_D + 2) * sizeof(float); }
 
 hipError_t launch_kv_attention(const KvParams &p, int cus, bool ws, float *part, unsigned *cnt, unsigned S, float *rpart, hipStream_t s) {
   if (p.rows == 0 || p.B == 0 || p.Hq == 0) return hipSuccess;
-  const uint64_t per = rows_per_seq(p);
-  if (per > 64) {
+  if (by_blocks(p, cus)) {
     const uint32_t items = block_items(p);
     const dim3 grid(items * p.Hkv * S), block(512);
     if (p.cap > 0.0f) hipLaunchKernelGGL((k_kv_attn_block<8, true>), grid, block, 0, s, p, items, S, rpart);
@@ -803,10 +843,9 @@ hipError_t launch_kv_attention(const KvParams &p, int cus, bool ws, float *part,
     hipLaunchKernelGGL(k_kv_attn_join, dim3((uint32_t)((threads + 255) / 256)), dim3(256), 0, s, p, S, rpart);
     return hipGetLastError();
   }
-  auto go = [&](auto kernel, int nw) { hipLaunchKernelGGL(kernel, dim3(cus), dim3(64 * nw), 0, s, p, ws ? 1u : 0u, part, cnt); };
-  if (per <= 16) p.cap > 0.0f ? go(k_kv_attn_split<1, 8, true>, 8) : go(k_kv_attn_split<1, 8, false>, 8);
-  else if (per <= 32) p.cap > 0.0f ? go(k_kv_attn_split<2, 8, true>, 8) : go(k_kv_attn_split<2, 8, false>, 8);
-  else p.cap > 0.0f ? go(k_kv_attn_split<4, 4, true>, 4) : go(k_kv_attn_split<4, 4, false>, 4);
+  const dim3 grid(cus), block(64 * KVA_NW);
+  if (p.cap > 0.0f) hipLaunchKernelGGL(k_kv_attn_split<true>, grid, block, 0, s, p, ws ? 1u : 0u, part, cnt);
+  else hipLaunchKernelGGL(k_kv_attn_split<false>, grid, block, 0, s, p, ws ? 1u : 0u, part, cnt);
   return hipGetLastError();
 }
 

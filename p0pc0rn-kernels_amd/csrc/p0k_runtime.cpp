@@ -1002,7 +1002,7 @@ int p0k_kv_attention(p0k_ctx *c, const p0k_kv_attn_args *a) {
   if (int rr = ws_allowed(c, &capturing, &ws)) return rr;
   if (ws) c->capture_ws = true;
   const int cus = [&] { std::lock_guard<std::mutex> lk(c->mu); return (int)c->tune.cus; }();
-  unsigned S = std::max(1u, p0k::kv_attention_runs(p, cus));
+  unsigned S = p0k::kv_attention_runs(p, cus);
   float *rpart = nullptr;
   if (S > 1) {
     // (no workspace to be had: one run)
