@@ -160,7 +160,7 @@ typedef struct p0k_attn_args {
  * starts rs * r + hs * h halves behind off (0: rs = 128, hs = rows * rs, the `heads` epilogue's layout; token-major:
  * rs = H * 128, hs = 128). Offsets 16-byte aligned, strides multiples of 8.
  *
- * p0k_batch: the rows of a call belong to B sequences, rows cu[b] .. cu[b + 1] - 1 to sequence b (int32, not decreasing,
+ * p0k_batch: the rows of a call belong to B sequences, rows cu[b] .. cu[b + 1] - 1 to sequence b (int32, must not decrease,
  * B + 1 of them); row r is that sequence's token t = pos[b] + r - cu[b] (int32). Rows outside [cu[0], cu[B]) are left as
  * they are. slot[b] (int32, optional: b) says which sequence of the cache it is. All three are read on the device, so a
  * captured graph serves other lengths when their contents change. A sequence with pos < 0 or a slot outside the cache has
@@ -235,7 +235,7 @@ typedef struct p0k_kv_read_args {
 /* kv_attention: O [rows][ldo] f16, head h at column h * 128 = softmax(scale q.k) v over the cached tokens j that the query
  * at token t sees: j <= t and, with a window, j > t - window or j < sinks. The cache holds the batch's own rows already
  * (p0k_kv_append comes first): sequence b has pos[b] + cu[b + 1] - cu[b] tokens. Query head h reads kv head h / (Hq / Hkv).
- * A row that sees nothing is 0. Zero fields: ldo = Hq * 128, scale = 1 / sqrt(128), window: none, cap: none (cap * tanh(s /
+ * A row that sees nothing is 0 (with offsets that decrease, rows may be left as they are). Zero fields: ldo = Hq * 128, scale = 1 / sqrt(128), window: none, cap: none (cap * tanh(s /
  * cap) otherwise). o: 8-byte aligned, ldo a multiple of 4. Pages wholly outside every row's window are not read. The keys
  * are divided over workgroups through a fixed workspace of the context (not in a capture begun by the caller). */
 typedef struct p0k_kv_attn_args {
@@ -362,7 +362,7 @@ int p0k_pack_f16(const float *W, uint64_t n, uint16_t *out);
 
 /* ---- HIP graphs: capture the context's stream (e.g. a decode step's gemm calls), then replay it with one launch.
  *      (The reference batches dispatches into command buffers, src/core/gpu.js:203-257; a graph is the HIP form.)
- *      Between begin and end only enqueueing calls may be made (p0k_gemm, p0k_rowstats, p0k_copy).
+ *      Between begin and end only enqueueing calls may be made (p0k_gemm, p0k_rowstats, p0k_copy, p0k_rope, p0k_kv_*).
  *      Workspaces cannot grow during a capture, so one call of each shape should be made before it. Without it, a call that
  *      cannot do without is refused ("must grow": rms / lnmod prompts, PixelNorm clips, decode with K split); one that
  *      can runs by another, usually slower plan: K of a prompt unsplit, the prologue of a decode or of a GroupNorm convolution

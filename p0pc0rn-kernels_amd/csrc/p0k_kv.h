@@ -48,7 +48,8 @@ struct RopeParams {
 };
 
 // what a sequence of the batch has in this call: rows r0 .. r0 + n - 1, its first token and its slot (ok: it has tokens)
-struct KvSeq { uint32_t r0, n, pos, slot; bool ok; };
+// (down: its rows end before they begin, the batch's offsets are none)
+struct KvSeq { uint32_t r0, n, pos, slot; bool ok, down; };
 
 #ifdef __HIPCC__
 __device__ __forceinline__ uint32_t kv_row0(const int32_t *cu, uint32_t b, uint32_t rows) {
@@ -61,6 +62,7 @@ __device__ __forceinline__ KvSeq kv_seq(const KvParams &p, uint32_t b) {
   const uint32_t r1 = kv_row0(p.cu, b + 1, p.rows);
   const int32_t pos = p.pos[b], slot = p.slot ? p.slot[b] : (int32_t)b;
   s.n = r1 > s.r0 ? r1 - s.r0 : 0u;
+  s.down = r1 < s.r0;
   s.ok = pos >= 0 && slot >= 0 && (uint32_t)slot < p.slots;
   s.pos = s.ok ? (uint32_t)pos : 0u;
   s.slot = s.ok ? (uint32_t)slot : 0u;
@@ -89,7 +91,7 @@ __device__ __forceinline__ KvItem kv_item(const KvParams &p, uint32_t item) {
   const uint32_t f = s.r0 / U + 2u * b;
   const uint64_t m = __ballot(lane < n && f <= item);
   const uint32_t k = m ? 63u - (uint32_t)__builtin_clzll(m) : 0u;
-  KvItem o;
+  KvItem o = {};
   o.s.r0 = __builtin_amdgcn_readlane(s.r0, k);
   o.s.n = __builtin_amdgcn_readlane(s.n, k);
   o.s.pos = __builtin_amdgcn_readlane(s.pos, k);
@@ -152,8 +154,8 @@ unsigned kv_attention_counters(int cus);
 hipError_t launch_rope(const RopeParams &p, hipStream_t s);
 hipError_t launch_kv_append(const KvParams &p, hipStream_t s);
 hipError_t launch_kv_read(const KvParams &p, hipStream_t s);
-// with many queries: runs into which a block's keys are divided where the blocks alone do not fill the GPU (1: not at all), and
-// the bytes that a run leaves
+// 0: the call takes the kernel over runs of keys; else the one over blocks of rows, and the runs into which a block's keys are
+// divided (more than 1 where the blocks alone do not fill the GPU); the bytes that a run leaves
 unsigned kv_attention_runs(const KvParams &p, int cus);
 uint64_t kv_attention_run_bytes(const KvParams &p);
 // ws: part / cnt may be used; S > 1: rpart holds S runs

@@ -114,6 +114,7 @@ __device__ __forceinline__ bool attn_split(const KvParams &p, uint32_t ws, float
   // (lane i knows sequence cb + i: what it has, and the units up to its end from the chunk's start)
   KvSeq ls;
   uint32_t cb = 0, sum = 0;
+  bool down = false;
   auto chunk = [&](uint32_t b0) {
     cb = b0;
     ls = KvSeq{};
@@ -123,13 +124,14 @@ __device__ __forceinline__ bool attn_split(const KvParams &p, uint32_t ws, float
       const KvWork w = kv_work<RB>(p, ls);
       t = w.units * w.blocks * p.Hkv;
     }
+    down = down || __any(ls.down);
     sum = wave_scan(t);
     return __builtin_amdgcn_readlane(sum, 63);
   };
   auto work = [&](uint32_t b) {                                                   // of sequence b
     if (b - cb >= 64) chunk(b & ~63u);
     const uint32_t i = b - cb;
-    KvSeq q;
+    KvSeq q = {};
     q.r0 = __builtin_amdgcn_readlane(ls.r0, i);
     q.n = __builtin_amdgcn_readlane(ls.n, i);
     q.pos = __builtin_amdgcn_readlane(ls.pos, i);
@@ -139,6 +141,7 @@ __device__ __forceinline__ bool attn_split(const KvParams &p, uint32_t ws, float
   };
   uint32_t T = chunk(0);
   for (uint32_t b0 = 64; b0 < p.B; b0 += 64) T += chunk(b0);
+  if (down) T = 0;                                // offsets that decrease: sequences could share rows, and T pass 32 bits
   // the sequence of unit u < T, and its first unit
   auto find = [&](uint32_t u, uint32_t *base) {
     uint32_t at = 0, all = cb == 0 ? __builtin_amdgcn_readlane(sum, 63) : chunk(0);
@@ -824,7 +827,8 @@ static uint32_t block_items(const KvParams &p) { return (uint32_t)((uint64_t)p.r
 // Runs of a block's keys: two workgroups for each CU between all blocks, eight at most (two chunks of 1145 queries after 12000
 // keys, 152 blocks: one run 456 us, two 349, three 327, four 315)
 unsigned kv_attention_runs(const KvParams &p, int cus) {
-  if (!by_blocks(p, cus) || p.max_pages < 8) return 1;
+  if (!by_blocks(p, cus)) return 0;
+  if (p.max_pages < 8) return 1;
   const uint64_t groups = (uint64_t)block_items(p) * p.Hkv;
   return groups >= 2u * cus ? 1u : std::min(8u, (unsigned)((2u * cus + groups - 1) / groups));
 }
@@ -832,7 +836,7 @@ uint64_t kv_attention_run_bytes(const KvParams &p) { return (uint64_t)p.rows * p
 
 hipError_t launch_kv_attention(const KvParams &p, int cus, bool ws, float *part, unsigned *cnt, unsigned S, float *rpart, hipStream_t s) {
   if (p.rows == 0 || p.B == 0 || p.Hq == 0) return hipSuccess;
-  if (by_blocks(p, cus)) {
+  if (S) {
     const uint32_t items = block_items(p);
     const dim3 grid(items * p.Hkv * S), block(512);
     if (p.cap > 0.0f) hipLaunchKernelGGL((k_kv_attn_block<8, true>), grid, block, 0, s, p, items, S, rpart);

@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256) void k_rope(RopeParams p, uint32_t hg) {
 
 // Heads a thread walks: all of them where the rows alone fill the GPU (2048 workgroups), else as few as do
 hipError_t launch_rope(const RopeParams &p, hipStream_t s) {
-  if (p.rows == 0 || p.H == 0) return hipSuccess;
+  if (p.rows == 0 || p.H == 0 || (p.cu && p.B == 0)) return hipSuccess;
   const uint32_t wgs = (p.rows + 15) / 16, groups = wgs >= 2048 ? 1 : (2048 + wgs - 1) / wgs;
   uint32_t hg = (p.H + groups - 1) / groups;
   hg = hg < 4 ? 4 : (hg + 3) / 4 * 4;

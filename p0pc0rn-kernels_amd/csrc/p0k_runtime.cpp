@@ -1000,10 +1000,10 @@ int p0k_kv_attention(p0k_ctx *c, const p0k_kv_attn_args *a) {
   std::lock_guard<std::mutex> order(c->enq);
   bool capturing, ws;
   if (int rr = ws_allowed(c, &capturing, &ws)) return rr;
-  if (ws) c->capture_ws = true;
   const int cus = [&] { std::lock_guard<std::mutex> lk(c->mu); return (int)c->tune.cus; }();
   unsigned S = p0k::kv_attention_runs(p, cus);
   float *rpart = nullptr;
+  if (S == 0 && ws) c->capture_ws = true;
   if (S > 1) {
     // (no workspace to be had: one run)
     if (int rr = WsSource{c, nullptr}.slices_if(0, S * p0k::kv_attention_run_bytes(p), &rpart)) return rr;

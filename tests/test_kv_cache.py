@@ -540,6 +540,40 @@ def test_batch_offsets_are_held_to_the_rows(cache):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [40, 600])
+def test_decreasing_offsets_end(cache, n):
+    """offsets that go up and down, so that sequences would share all rows: the calls end, inside their buffers"""
+    rng = np.random.default_rng(15)
+    B = 200
+    c = cache(2, B, 12)
+    x = c.up(rng.standard_normal((8, n, D)).astype(np.float16))
+    o = c.up(np.zeros((n, 8 * D), np.float16))
+    cu = np.where(np.arange(B + 1) % 2, n, 0).astype(np.int32)
+    for pos in (0, 700):
+        b = {"pos": c.up(np.full(B, pos, np.int32)), "cu": c.up(cu), "B": B, "rows": n}
+        c.dev.kv_append({"cache": c.c, "batch": b, "k": x, "v": x})
+        c.dev.kv_attention({"cache": c.c, "batch": b, "q": x, "o": o, "Hq": 8})
+        c.dev.kv_attention({"cache": c.c, "batch": b, "q": x, "o": o, "Hq": 8, "window": 70, "sinks": 3})
+        c.dev.rope({"x": x, "H": 8, "batch": b})
+        c.dev.done()
+
+
+@pytest.mark.gpu
+def test_nothing_to_do(cache):
+    """no sequences, no rows: the calls are accepted and write nothing"""
+    c = cache(2, 2, 4)
+    x, o = c.up(np.full((8, 6, D), 0x1234, np.uint16)), c.up(np.full((6, 8 * D), 0x1234, np.uint16))
+    cu = c.up(np.zeros(3, np.int32))
+    for B, rows in ((0, 6), (2, 0), (2, 6)):
+        b = {"pos": cu, "cu": cu, "B": B, "rows": rows}
+        c.dev.kv_append({"cache": c.c, "batch": b, "k": x, "v": x})
+        c.dev.kv_read({"cache": c.c, "batch": b, "len": cu, "k": x, "v": o})
+        c.dev.kv_attention({"cache": c.c, "batch": b, "q": x, "o": o, "Hq": 8})
+        c.dev.rope({"x": x, "H": 8, "batch": b})
+    assert np.all(c.dev.read(x, np.uint16) == 0x1234) and np.all(c.dev.read(o, np.uint16) == 0x1234)
+
+
+@pytest.mark.gpu
 def test_many_sequences(cache):
     """more sequences than one step of the search over the batch takes, most of them without rows"""
     rng = np.random.default_rng(14)
@@ -724,6 +758,82 @@ def test_decode_loop_in_a_graph(dev):
         for b in (qkv, rot, pos, cu, o):
             dev.free(b)
         c.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 700])
+def test_capture_begun_by_the_caller(cache, n):
+    """in a capture that the caller began the attention does without workspaces (whole groups, one run of keys): the same
+    values, with the context's own calls between the replays"""
+    hip = C.CDLL("libamdhip64.so")
+    rng = np.random.default_rng(31)
+    c = cache(2, 2, 40)
+    dev = c.dev
+    fill(c, [1500 + n, 200 + n], rng)
+    b, cu = c.batch([1500, 200], [n, n], [0, 1])
+    q = rng.standard_normal((b["rows"], 8, D)).astype(np.float16)
+    qb, o = c.rows(q, False), c.up(np.zeros((b["rows"], 8 * D), np.float16))
+    a = {"cache": c.c, "batch": b, "q": qb, "o": o, "Hq": 8}
+    stream = C.c_void_p(p0k.lib().p0k_ctx_stream(dev.ctx))
+    graph, exe = C.c_void_p(), C.c_void_p()
+    assert hip.hipStreamBeginCapture(stream, 1) == 0                 # thread-local capture mode
+    try:
+        dev.kv_attention(a)
+    finally:
+        assert hip.hipStreamEndCapture(stream, C.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(C.byref(exe), graph, None, None, C.c_size_t(0)) == 0
+    try:
+        for i in range(3):
+            dev.upload(np.zeros((b["rows"], 8 * D), np.float16), o)
+            assert hip.hipGraphLaunch(exe, stream) == 0
+            dev.done()
+            got = dev.read(o, np.float16, b["rows"] * 8 * D).reshape(-1, 8, D).astype(np.float64)
+            for s, p in enumerate((1500, 200)):
+                k, v = c.ref.held(s, read=False)
+                w, tol = attend_ref(q[cu[s]:cu[s + 1]], p, k, v, 4)
+                assert np.all(np.abs(got[cu[s]:cu[s + 1]] - w) <= tol)
+            dev.kv_attention(a)
+    finally:
+        hip.hipGraphExecDestroy(exe)
+        hip.hipGraphDestroy(graph)
+
+
+@pytest.mark.gpu
+def test_two_graphs_share_the_workspaces(cache):
+    """graphs of the two kernels and of both block sizes, replayed in turn with eager calls in between and positions changed"""
+    rng = np.random.default_rng(32)
+    c = cache(4, 6, 70)
+    dev = c.dev
+    fill(c, [4400] * 6, rng)
+    calls, graphs = [], []
+    for n in (1, 6, 300):                                            # one of each: 16 rows, 32 rows, blocks of 256
+        b, cu = c.batch([4400 - n] * 6, [n] * 6, range(6))
+        q = rng.standard_normal((b["rows"], 16, D)).astype(np.float16)
+        o = c.up(np.zeros((b["rows"], 16 * D), np.float16))
+        a = {"cache": c.c, "batch": b, "q": c.rows(q, False), "o": o, "Hq": 16}
+        dev.kv_attention(a)
+        want = dev.read(o, np.uint16)
+        k, v = c.ref.held(2, read=False)
+        w, tol = attend_ref(q[cu[2]:cu[3]], 4400 - n, k, v, 4)
+        got = want.view(np.float16)[:b["rows"] * 16 * D].reshape(-1, 16, D)[cu[2]:cu[3]].astype(np.float64)
+        assert np.all(np.abs(got - w) <= tol)
+        dev.graph_begin()
+        dev.kv_attention(a)
+        graphs.append(dev.graph_end())
+        calls.append((a, b, o, want, n))
+    try:
+        for i in (0, 1, 2, 1, 0, 2, 2, 0, 1):
+            a, b, o, want, n = calls[i]
+            dev.upload(np.zeros_like(want), o)
+            dev.upload(np.full(6, 1000 - n, np.int32), b["pos"])
+            dev.graph_launch(graphs[i])                              # (another length: the plan is made on the device)
+            dev.kv_attention(calls[(i + 1) % 3][0])
+            dev.upload(np.full(6, 4400 - n, np.int32), b["pos"])
+            dev.graph_launch(graphs[i])
+            np.testing.assert_array_equal(dev.read(o, np.uint16), want)
+    finally:
+        for g in graphs:
+            dev.graph_destroy(g)
 
 
 @pytest.mark.gpu
