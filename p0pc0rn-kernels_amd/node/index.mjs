@@ -255,6 +255,72 @@ function attention(gpu, a) {
     scale: a.scale || 0, cap: a.cap || 0 });
 }
 
+// ------------------------------------------------------------------ rotary positions, 8-bit key / value cache (no counterpart
+// in the reference; include/p0k.h has the definitions). Rows: {buf, off, rs, hs}; batch: {pos, cu, slot, B, rows}, its buffers
+// {buf, off} of int32 or the buffer itself.
+const operand = (d, name, x) => {
+  if (!x) return;
+  if (!x.buf) x = { buf: x };
+  Object.assign(d, { [name + '_buf']: ptrOf(x.buf), [name + '_off']: x.off || 0, [name + '_size']: sizeOf(x.buf),
+    [name + '_rs']: x.rs || 0, [name + '_hs']: x.hs || 0 });
+};
+function batchDesc(d, b) {
+  for (const n of ['pos', 'cu', 'slot']) operand(d, n, b[n]);
+  d.B = b.B || 0; d.rows = b.rows;
+}
+function cacheDesc(a) {
+  const d = { pages: a.cache.pages, slots: a.cache.slots, max_pages: a.cache.maxPages, Hkv: a.cache.Hkv };
+  for (const n of ['code', 'scale', 'tail', 'table']) operand(d, n, a.cache[n]);
+  batchDesc(d, a.batch);
+  return d;
+}
+
+/** rope(gpu, {x, y (default x: in place), H, batch, rd, mode: 'interleaved' | 'half', theta, scaling: {kind: 'linear' | 'bands',
+ *  factor, orig, low, high}, freqs, mscale}): rotary positions */
+function rope(gpu, a) {
+  const sc = a.scaling || {};
+  const d = { H: a.H, rd: a.rd || 0, mode: a.mode === 'half' ? 1 : 0, scaling: { linear: 1, bands: 2 }[sc.kind] || 0, theta: a.theta || 0,
+    factor: sc.factor || 0, orig: sc.orig || 0, low: sc.low || 0, high: sc.high || 0, mscale: a.mscale || 0 };
+  operand(d, 'x', a.x);
+  operand(d, 'y', a.y || a.x);
+  batchDesc(d, a.batch);
+  call(addon().rope, gpu.ctx, d, a.freqs ? Float64Array.from(a.freqs) : undefined);
+}
+
+/** kvCache(gpu, {Hkv, pages, slots, maxPages, table}): the buffers of a cache, `pages` pages of 64 tokens for `slots` sequences of
+ *  up to maxPages blocks. table: Int32 [slots][maxPages] buffer of page numbers (default: sequence s owns pages s * maxPages on) */
+function kvCache(gpu, o) {
+  const [code, scale, tail] = call(addon().kvBytes, o.pages, o.slots, o.Hkv);
+  let table = o.table;
+  if (!table) table = gpu.upload(Int32Array.from({ length: o.slots * o.maxPages }, (_, i) => (i < o.pages ? i : -1)), 'kv table');
+  return { code: gpu.buffer(code, 'kv codes'), scale: gpu.buffer(scale, 'kv scales'), tail: gpu.buffer(tail, 'kv tail'), table,
+    pages: o.pages, slots: o.slots, maxPages: o.maxPages, Hkv: o.Hkv };
+}
+
+/** kvAppend(gpu, {cache, batch, k, v}): rows of K / V into the cache */
+function kvAppend(gpu, a) {
+  const d = cacheDesc(a);
+  operand(d, 'k', a.k);
+  operand(d, 'v', a.v);
+  call(addon().kvAppend, gpu.ctx, d);
+}
+
+/** kvRead(gpu, {cache, batch, len, k, v}): cached rows back as f16 */
+function kvRead(gpu, a) {
+  const d = cacheDesc(a);
+  for (const n of ['len', 'k', 'v']) operand(d, n, a[n]);
+  call(addon().kvRead, gpu.ctx, d);
+}
+
+/** kvAttention(gpu, {cache, batch, q, o: {buf, off, ld}, Hq, window, sinks, scale, cap}): attention over the cache */
+function kvAttention(gpu, a) {
+  const d = Object.assign(cacheDesc(a), { Hq: a.Hq, ldo: a.o.ld || 0, window: a.window || 0, sinks: a.sinks || 0, scale: a.scale || 0,
+    cap: a.cap || 0 });
+  operand(d, 'q', a.q);
+  operand(d, 'o', a.o);
+  call(addon().kvAttention, gpu.ctx, d);
+}
+
 // ------------------------------------------------------------------ conv prologue statistics (src/ops/video.js, misc.js)
 /** pixstats(gpu, {x: {buf, off}, r: {buf}, V, C, eps = 1e-8, ro}): r[ro + v] = 1 / sqrt(mean_c x[v][c]^2 + eps) */
 function pixstats(gpu, a) {
@@ -542,7 +608,7 @@ function encodeRows(enc, W, rows, K) {
 
 export {
   MB, GpuError, createGpu, Gpu, f2h, h2f, toF16, fromF16,
-  gemm, gemmPlan, gemmDesc, DEFAULT_TILE, rowstats, attention, pixstats, gnPartBytes, gnPartial, gnFinalize, groupnormStats,
+  gemm, gemmPlan, gemmDesc, DEFAULT_TILE, rowstats, attention, rope, kvCache, kvAppend, kvRead, kvAttention, pixstats, gnPartBytes, gnPartial, gnFinalize, groupnormStats,
   TUNE_TABLE, tuneEntry, defaultTune, calibrate,
   MANIFEST_FORMAT, loadWeights, uploadWeights,
   packQ4, packQ8, packF16, packF32, encodedBytes, tileBytes, encodeRows,

@@ -4,7 +4,7 @@
  * every argument check happens in libp0k, whose message becomes the thrown Error's message.
  *
  * Exports: ctxCreate, ctxDestroy, deviceInfo, alloc, free, upload, download, copy, sync, poolStats, drainPool,
- *          gemm, gemmCheck, selectTile, rowstats, attention, pixstats, gn, gnPartBytes, packQ4, packQ8, packF16, tensorBytes,
+ *          gemm, gemmCheck, selectTile, rowstats, attention, rope, kvBytes, kvAppend, kvRead, kvAttention, pixstats, gn, gnPartBytes, packQ4, packQ8, packF16, tensorBytes,
  *          lastError, abiVersion
  * (N-API version 6 or later: BigInt support; Node 12.17+).
  */
@@ -426,6 +426,132 @@ static napi_value gn(napi_env env, napi_callback_info info) {   /* (ctx, desc, w
   return mk_num(env, nwg);
 }
 
+/* ------------------------------------------------------------------ rotary positions, 8-bit key / value cache */
+static int field_f64(napi_env env, napi_value o, const char *name, double *out) {
+  napi_value v;
+  napi_valuetype t;
+  *out = 0.0;
+  if (napi_get_named_property(env, o, name, &v) != napi_ok) return 0;
+  napi_typeof(env, v, &t);
+  if (t == napi_undefined || t == napi_null) return 1;
+  return napi_get_value_double(env, v, out) == napi_ok;
+}
+/* fields <name>_buf, _off, _size and, with strides, _rs, _hs */
+static int operand(napi_env env, napi_value o, const char *name, const void **buf, uint64_t *off, uint64_t *size, uint64_t *rs, uint64_t *hs) {
+  static const char *const part[] = {"_buf", "_off", "_size", "_rs", "_hs"};
+  uint64_t v[5] = {0};
+  char f[32];
+  for (int i = 0; i < (rs ? 5 : 3); i++) {
+    snprintf(f, sizeof f, "%s%s", name, part[i]);
+    if (!field_u64(env, o, f, &v[i])) { napi_throw_type_error(env, NULL, f); return 0; }
+  }
+  *buf = (const void *)(uintptr_t)v[0]; *off = v[1]; *size = v[2];
+  if (rs) { *rs = v[3]; *hs = v[4]; }
+  return 1;
+}
+#define OPERAND(o, name, s) operand(env, o, #name, (const void **)&(s).name##_buf, &(s).name##_off, &(s).name##_size, NULL, NULL)
+#define ROWS(o, name, s) operand(env, o, #name, (const void **)&(s).name##_buf, &(s).name##_off, &(s).name##_size, &(s).name##_rs, &(s).name##_hs)
+static int fields_u32(napi_env env, napi_value o, const char *const *names, uint32_t *const *dst, int n) {
+  for (int i = 0; i < n; i++) {
+    uint64_t v;
+    if (!field_u64(env, o, names[i], &v) || v > 0xffffffffu) { napi_throw_type_error(env, NULL, names[i]); return 0; }
+    *dst[i] = (uint32_t)v;
+  }
+  return 1;
+}
+static int batch_of(napi_env env, napi_value o, p0k_batch *b) {
+  return OPERAND(o, pos, *b) && OPERAND(o, cu, *b) && OPERAND(o, slot, *b) &&
+         fields_u32(env, o, (const char *const[]){"B", "rows"}, (uint32_t *const[]){&b->B, &b->rows}, 2);
+}
+static int cache_of(napi_env env, napi_value o, p0k_kv_cache *c) {
+  return OPERAND(o, code, *c) && OPERAND(o, scale, *c) && OPERAND(o, tail, *c) && OPERAND(o, table, *c) &&
+         fields_u32(env, o, (const char *const[]){"pages", "slots", "max_pages", "Hkv"},
+                    (uint32_t *const[]){&c->pages, &c->slots, &c->max_pages, &c->Hkv}, 4);
+}
+
+static napi_value rope(napi_env env, napi_callback_info info) {   /* (ctx, desc, freqs Float64Array | undefined) */
+  napi_value argv[3];
+  if (!get_args(env, info, 3, argv)) return NULL;
+  napi_value o = argv[1];
+  p0k_rope_args a;
+  memset(&a, 0, sizeof a);
+  a.struct_size = sizeof a;
+  uint32_t mode = 0, scaling = 0;
+  if (!ROWS(o, x, a) || !ROWS(o, y, a) || !batch_of(env, o, &a.batch) ||
+      !fields_u32(env, o, (const char *const[]){"H", "rd", "mode", "scaling"}, (uint32_t *const[]){&a.H, &a.rd, &mode, &scaling}, 4))
+    return NULL;
+  a.mode = (int32_t)mode;
+  a.scaling = (int32_t)scaling;
+  if (!field_f64(env, o, "theta", &a.theta) || !field_f64(env, o, "factor", &a.factor) || !field_f64(env, o, "orig", &a.orig) ||
+      !field_f64(env, o, "low", &a.low) || !field_f64(env, o, "high", &a.high) || !field_f32(env, o, "mscale", &a.mscale)) {
+    napi_throw_type_error(env, NULL, "field theta / factor / orig / low / high / mscale");
+    return NULL;
+  }
+  void *f = NULL;
+  size_t len = 0;
+  if (get_bytes(env, argv[2], &f, &len)) {
+    if (len != (a.rd ? a.rd : 128u) / 2 * sizeof(double)) { napi_throw_type_error(env, NULL, "freqs: rd / 2 numbers"); return NULL; }
+    a.freqs = (const double *)f;
+  }
+  int r = p0k_rope(get_ctx(env, argv[0]), &a);
+  return r ? throw_p0k(env, r) : undef(env);
+}
+
+static napi_value kvBytes(napi_env env, napi_callback_info info) {   /* (pages, slots, Hkv) -> [codes, scales, tail] */
+  napi_value argv[3], out;
+  uint64_t v[3];
+  if (!get_args(env, info, 3, argv)) return NULL;
+  for (int i = 0; i < 3; i++)
+    if (!to_u64(env, argv[i], &v[i]) || v[i] > 0xffffffffu) { napi_throw_type_error(env, NULL, "pages, slots, Hkv"); return NULL; }
+  CHECK_NAPI(env, napi_create_array_with_length(env, 3, &out));
+  CHECK_NAPI(env, napi_set_element(env, out, 0, mk_num(env, (double)p0k_kv_code_bytes((uint32_t)v[0], (uint32_t)v[2]))));
+  CHECK_NAPI(env, napi_set_element(env, out, 1, mk_num(env, (double)p0k_kv_scale_bytes((uint32_t)v[0], (uint32_t)v[2]))));
+  CHECK_NAPI(env, napi_set_element(env, out, 2, mk_num(env, (double)p0k_kv_tail_bytes((uint32_t)v[1], (uint32_t)v[2]))));
+  return out;
+}
+
+static napi_value kvAppend(napi_env env, napi_callback_info info) {   /* (ctx, desc) */
+  napi_value argv[2];
+  if (!get_args(env, info, 2, argv)) return NULL;
+  p0k_kv_append_args a;
+  memset(&a, 0, sizeof a);
+  a.struct_size = sizeof a;
+  if (!cache_of(env, argv[1], &a.cache) || !batch_of(env, argv[1], &a.batch) || !ROWS(argv[1], k, a) || !ROWS(argv[1], v, a)) return NULL;
+  int r = p0k_kv_append(get_ctx(env, argv[0]), &a);
+  return r ? throw_p0k(env, r) : undef(env);
+}
+
+static napi_value kvRead(napi_env env, napi_callback_info info) {   /* (ctx, desc) */
+  napi_value argv[2];
+  if (!get_args(env, info, 2, argv)) return NULL;
+  p0k_kv_read_args a;
+  memset(&a, 0, sizeof a);
+  a.struct_size = sizeof a;
+  if (!cache_of(env, argv[1], &a.cache) || !batch_of(env, argv[1], &a.batch) || !OPERAND(argv[1], len, a) || !ROWS(argv[1], k, a) ||
+      !ROWS(argv[1], v, a))
+    return NULL;
+  int r = p0k_kv_read(get_ctx(env, argv[0]), &a);
+  return r ? throw_p0k(env, r) : undef(env);
+}
+
+static napi_value kvAttention(napi_env env, napi_callback_info info) {   /* (ctx, desc) */
+  napi_value argv[2];
+  if (!get_args(env, info, 2, argv)) return NULL;
+  napi_value o = argv[1];
+  p0k_kv_attn_args a;
+  memset(&a, 0, sizeof a);
+  a.struct_size = sizeof a;
+  if (!cache_of(env, o, &a.cache) || !batch_of(env, o, &a.batch) || !ROWS(o, q, a) || !OPERAND(o, o, a) ||
+      !fields_u32(env, o, (const char *const[]){"ldo", "Hq", "window", "sinks"}, (uint32_t *const[]){&a.ldo, &a.Hq, &a.window, &a.sinks}, 4))
+    return NULL;
+  if (!field_f32(env, o, "scale", &a.scale) || !field_f32(env, o, "cap", &a.cap)) {
+    napi_throw_type_error(env, NULL, "field scale / cap");
+    return NULL;
+  }
+  int r = p0k_kv_attention(get_ctx(env, argv[0]), &a);
+  return r ? throw_p0k(env, r) : undef(env);
+}
+
 static napi_value attention(napi_env env, napi_callback_info info) {   /* (ctx, desc) -> flops */
   napi_value argv[2];
   if (!get_args(env, info, 2, argv)) return NULL;
@@ -537,6 +663,7 @@ static napi_value init(napi_env env, napi_value exports) {
       {"selectTile", selectTile}, {"rowstats", rowstats}, {"packQ4", packQ4}, {"packQ8", packQ8},
       {"packF16", packF16}, {"tensorBytes", tensorBytes}, {"lastError", lastError}, {"abiVersion", abiVersion},
       {"pixstats", pixstats}, {"gn", gn}, {"gnPartBytes", gnPartBytes}, {"attention", attention},
+      {"rope", rope}, {"kvBytes", kvBytes}, {"kvAppend", kvAppend}, {"kvRead", kvRead}, {"kvAttention", kvAttention},
   };
   for (size_t i = 0; i < sizeof fns / sizeof fns[0]; i++) {
     napi_value f;
