@@ -134,6 +134,10 @@ struct Part {
   }
 };
 
+// A head's codes in LDS: runs of 16 pieces (256 bytes: all banks), each moved on by a piece, since the words that a wave writes or
+// reads at once lie at the same places of 16 runs
+__device__ __forceinline__ uint32_t kv_lds(uint32_t code) { return code + (code >> 8) * 16; }
+
 template <int KV>
 __device__ void append_block(const KvParams &p, const KvSeq &s, uint32_t blk, uint32_t k0, uint32_t end, uint32_t h, uint8_t *sC, float *sMax) {
   const uint32_t tid = threadIdx.x;
@@ -185,11 +189,11 @@ __device__ void append_block(const KvParams &p, const KvSeq &s, uint32_t blk, ui
         if (have) *(u32x4 *)(codes + kv_kcode(part.tok(0), part.d(2 * i))) = (u32x4){w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; j++) *(uint32_t *)(sC + kv_vcode(part.tok(0), part.d(0) + j)) = w[j];
+      for (int j = 0; j < 8; j++) *(uint32_t *)(sC + kv_lds(kv_vcode(part.tok(0), part.d(0) + j))) = w[j];
       __syncthreads();
       if (have) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) *(u32x4 *)(codes + 16 * (tid + 256 * i)) = *(const u32x4 *)(sC + 16 * (tid + 256 * i));
+        for (int i = 0; i < 2; i++) *(u32x4 *)(codes + 16 * (tid + 256 * i)) = *(const u32x4 *)(sC + kv_lds(16 * (tid + 256 * i)));
       }
     }
     if (have && tid == 0) p.scales[kv_scale_at(p, page, h, KV)] = sc;
@@ -247,11 +251,11 @@ __device__ void read_block(const KvParams &p, const KvSeq &s, uint32_t blk, uint
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 2; i++) *(u32x4 *)(sC + 16 * (tid + 256 * i)) = *(const u32x4 *)(codes + 16 * (tid + 256 * i));
+      for (int i = 0; i < 2; i++) *(u32x4 *)(sC + kv_lds(16 * (tid + 256 * i))) = *(const u32x4 *)(codes + 16 * (tid + 256 * i));
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const uint32_t w = *(const uint32_t *)(sC + kv_vcode(part.tok(0), part.d(0) + j));
+        const uint32_t w = *(const uint32_t *)(sC + kv_lds(kv_vcode(part.tok(0), part.d(0) + j)));
 #pragma unroll
         for (int i = 0; i < 4; i++) x[i][j] = kv_value(w, i, sc);
       }
