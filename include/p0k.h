@@ -176,8 +176,9 @@ typedef struct p0k_batch {
  * int8 codes of each kv head's 64 x 128 keys and values with one fp32 scale each (value = code * scale). Block k of
  * sequence s is page table[s][k] (int32). The block that a sequence is still filling and the one before it are held in
  * f16 in its tail. Buffers: p0k_kv_code_bytes / p0k_kv_scale_bytes / p0k_kv_tail_bytes; their inner layout is the
- * library's. Pages of whole blocks may be shared by sequences. A table entry outside [0, pages): the block is not there
- * (not written, not seen, read back as zeros); it may stay unset until the block before it is whole. */
+ * library's. Pages of whole blocks may be shared by sequences, as long as none of them goes back into such a block. A table
+ * entry outside [0, pages): the block is not there (not written, not seen, read back as zeros). The page of a block is written
+ * when the block becomes whole; until then its entry may stay unset. */
 typedef struct p0k_kv_cache {
   void *code_buf; uint64_t code_off, code_size;           /* codes, tail: 16-byte aligned; scales: 8-byte */
   float *scale_buf; uint64_t scale_off, scale_size;
@@ -235,9 +236,11 @@ typedef struct p0k_kv_read_args {
 /* kv_attention: O [rows][ldo] f16, head h at column h * 128 = softmax(scale q.k) v over the cached tokens j that the query
  * at token t sees: j <= t and, with a window, j > t - window or j < sinks. The cache holds the batch's own rows already
  * (p0k_kv_append comes first): sequence b has pos[b] + cu[b + 1] - cu[b] tokens. Query head h reads kv head h / (Hq / Hkv).
- * A row that sees nothing is 0 (with offsets that decrease, rows may be left as they are). Zero fields: ldo = Hq * 128, scale = 1 / sqrt(128), window: none, cap: none (cap * tanh(s /
- * cap) otherwise). o: 8-byte aligned, ldo a multiple of 4. Pages wholly outside every row's window are not read. The keys
- * are divided over workgroups through a fixed workspace of the context (not in a capture begun by the caller). */
+ * A row that sees nothing is 0 (with offsets that decrease, rows may be left as they are). Zero fields: ldo = Hq * 128,
+ * scale = 1 / sqrt(128), window: none, cap: none (cap * tanh(s / cap) otherwise); scale in [2^-40, 2^40], cap in [2^-20,
+ * 2^20]. o: 8-byte aligned, ldo a multiple of 4. Pages wholly outside every row's window are not read. The keys are divided
+ * over workgroups through workspaces of the context: a fixed one, and with many queries after a long cache the one of split
+ * prompts (in a capture only where it has grown to the size before; neither in a capture begun by the caller). */
 typedef struct p0k_kv_attn_args {
   uint32_t struct_size;
   p0k_kv_cache cache;

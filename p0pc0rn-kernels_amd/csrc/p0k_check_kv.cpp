@@ -137,7 +137,7 @@ int prepare_kv_attention(const p0k_kv_attn_args *a, KvParams *out, std::string *
   NEED(a->sinks == 0 || a->window != 0, "kv_attention: sinks without a window");
   // (a masked score is -1e30 before it is scaled, and has to stay far below the others)
   NEED(a->scale == 0.0f || (a->scale >= 0x1p-40f && a->scale <= 0x1p40f), "kv_attention: scale must be in [2^-40, 2^40] (0: 1 / sqrt(128))");
-  NEED(std::isfinite(a->cap) && a->cap >= 0.0f, "kv_attention: cap must be positive (0: none)");
+  NEED(a->cap == 0.0f || (a->cap >= 0x1p-20f && a->cap <= 0x1p20f), "kv_attention: cap must be in [2^-20, 2^20] (0: none)");
   CHECK(check_heads(err, "kv_attention", "q", a->q_buf, a->q_off, a->q_size, a->q_rs, a->q_hs, o.rows, a->Hq, false, &o.krs, &o.khs));
   NEED(a->o_buf != nullptr, "kv_attention: missing o buffer");
   o.ldo = a->ldo ? a->ldo : a->Hq * 128;

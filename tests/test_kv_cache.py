@@ -308,6 +308,9 @@ def test_attention_and_rope_refusals():
     refused("attend", "sinks without", sinks=4)
     refused("attend", "scale", scale=-1.0)
     refused("attend", "cap", cap=float("nan"))
+    refused("attend", "cap", cap=1e-30)
+    refused("attend", "scale", scale=1e-20)
+    refused("attend", "scale", scale=float("inf"))
     refused("attend", "o needs", o={"buf": _host(6 * 4 * D - 1, np.float16)})
     refused("attend", "covering", o={"buf": _host(6 * 4 * D, np.float16), "ld": 508})
     refused("rope", "even and at most", rd=130)
