@@ -352,6 +352,17 @@ __device__ __forceinline__ bool attn_split(const KvParams &p, uint32_t ws, float
       }
     };
 
+    // the open block's first unit is asked for before all others (with blocks of 32 rows there are no registers to hold it)
+    f16x8 ko[8], vo[8];
+    const uint32_t o0 = i0 < w.io ? w.io : i0;
+    auto open = [&](uint32_t i, uint32_t kv, f16x8 *to) {
+      const uint32_t un = unit_of(i);
+      const u16 *t = p.tail + kv_tail_at(p, w.s.slot, un >> 1, hk, kv) + (un & 1) * (KV_HEAD / 2) + lane * 8;
+#pragma unroll
+      for (int j = 0; j < 8; j++) to[j] = *(const f16x8 *)(t + 512 * j);
+    };
+    if (NB == 1 && o0 < i1) { open(o0, 0, ko); open(o0, 1, vo); }
+
     // whole blocks, up to 64 units ahead: lane i knows unit c0 + i's page and scales
     constexpr uint32_t NONE = 0xffffffffu;
     const uint32_t ic = i1 < w.io ? i1 : w.io;
@@ -388,16 +399,21 @@ __device__ __forceinline__ bool attn_split(const KvParams &p, uint32_t ws, float
       }
     }
     // the open block, in f16
-    for (uint32_t i = i0 < w.io ? w.io : i0; i < i1; i++) {
+    for (uint32_t i = o0; i < i1; i++) {
       const uint32_t un = unit_of(i);
-      const u16 *kt = p.tail + kv_tail_at(p, w.s.slot, un >> 1, hk, 0) + (un & 1) * (KV_HEAD / 2) + lane * 8, *vt = kt + KV_HEAD;
-      step(un, 1.0f, 1.0f, false, [&](int tt, int s) { return *(const f16x8 *)(kt + 512 * (4 * tt + s)); }, [] {},
+      if (NB != 1 && i == o0) open(i, 0, ko);
+      step(un, 1.0f, 1.0f, false, [&](int tt, int s) { return ko[4 * tt + s]; },
+           [&] {
+             if (NB != 1) open(i, 1, vo);
+             if (i + 1 < i1) open(i + 1, 0, ko);
+           },
            [&](int d) {
-             f16x8 v = *(const f16x8 *)(vt + 512 * d);
+             f16x8 v = vo[d];
 #pragma unroll
              for (int j = 0; j < 8; j++) v[j] = un * 32 + 16 * (j >> 2) + 4 * q4 + (j & 3) < w.end ? v[j] : (f16)0.0f;
              return v;
            });
+      if (NB == 1 && i + 1 < i1) open(i + 1, 1, vo);
     }
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
