@@ -92,8 +92,8 @@ __device__ __forceinline__ float rlf(float v, uint32_t l) { return __uint_as_flo
 // in f16; the scales stay in fp32: the keys' multiplies the scores, and O is held in units of the current block's value scale.
 // P is rounded to f16 (the products have no wider operand at this rate); sums, maxima and O are fp32.
 //
-// HBM-bound: 48 sequences of 900 to 6000 tokens, 8 kv heads (349 MB) 66 us, of which the keys' stream takes 50 (7 TB/s); one
-// sequence of 3777 tokens (7.8 MB) 9.7 us: about 2 us until the first codes are asked for, 1.4 for a unit, 6 for the exchanges.
+// HBM-bound: 48 sequences of 900 to 6000 tokens, 8 kv heads (349 MB) 63 us, of which the keys' stream takes 50 (7 TB/s); one
+// sequence of 3777 tokens (7.8 MB) 9.8 us: about 2 us until the first codes are asked for, 1.4 for a unit, 6 for the exchanges.
 // NB: blocks of 16 or 32 rows. 16 read the keys of 17 and more rows twice and more, but start and end sooner; the result is
 // false (and nothing done) where 32 are the better choice, see k_kv_attn_split.
 constexpr int KVA_NW = 8;                         // waves of a workgroup
@@ -352,7 +352,8 @@ __device__ __forceinline__ bool attn_split(const KvParams &p, uint32_t ws, float
       }
     };
 
-    // the open block's first unit is asked for before all others (with blocks of 32 rows there are no registers to hold it)
+    // the open block's first unit is asked for before all others (48 sequences: 66 -> 63 us; with blocks of 32 rows there are
+    // no registers to hold it)
     f16x8 ko[8], vo[8];
     const uint32_t o0 = i0 < w.io ? w.io : i0;
     auto open = [&](uint32_t i, uint32_t kv, f16x8 *to) {
