@@ -20,10 +20,10 @@ __device__ __forceinline__ uint32_t kv_bytes(uint32_t a, uint32_t b, uint32_t c,
   return perm(perm(d, c, 0x0c0c0400u), perm(b, a, 0x0c0c0400u), 0x05040100u);
 }
 // The bytes (code + 128) of a thread's 32 values, eight words of four: of consecutive d (keys) or of the four tokens of a d
-// (values). x / s is estimated as x rs, off by less than 2^-15, and the sum with 2^23 + 128 rounds it to the nearest integer.
-// Where an estimate of the wave lies within that of a border, all of them are settled exactly: x - c s takes no rounding where
-// it is near s / 2 (x has 11 bits and is at least s / 2 there, the difference needs no more than 24), and ties go to the even
-// code.
+// (values). x / s is estimated as x rs, off by less than 2^-16 (127 x 2^-24 of rs and 2^-18 of the product), and the sum with
+// 2^23 + 128 rounds it to the nearest integer. Where an estimate of the wave lies within that of a border, all of them are
+// settled exactly: x - c s takes no rounding where it is near s / 2 (x has 11 bits and is at least s / 2 there, the difference
+// needs no more than 24), and ties go to the even code.
 template <int KV>
 __device__ __forceinline__ void kv_codes(const u16x8 *x, float s, uint32_t *w) {
   const float rs = 1.0f / s, big = 8388608.0f + 128.0f;
@@ -40,7 +40,7 @@ __device__ __forceinline__ void kv_codes(const u16x8 *x, float s, uint32_t *w) {
     }
     w[g] = kv_bytes(__float_as_uint(z[0]), __float_as_uint(z[1]), __float_as_uint(z[2]), __float_as_uint(z[3]));
   }
-  if (__any(far > 0.5f - 0x1p-15f)) {
+  if (__any(far > 0.5f - 0x1p-16f)) {
     const float h = 0.5f * s;
 #pragma unroll
     for (int g = 0; g < 8; g++) {

@@ -840,6 +840,47 @@ def test_two_graphs_share_the_workspaces(cache):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 300])
+def test_graph_through_another_context(dev, n):
+    """a graph whose attention uses its context's workspaces: launched through another context it is ordered with the calls of
+    its own, and refused once that is gone"""
+    rng = np.random.default_rng(33)
+    own = p0k.Device(0)
+    g = None
+    try:
+        c = Cache(own, 4, 3, 40)
+        fill(c, [2300] * 3, rng)
+        calls = []
+        for m in (n, n + 1):
+            b, _ = c.batch([2300 - m] * 3, [m] * 3, range(3))
+            q = rng.standard_normal((b["rows"], 16, D)).astype(np.float16)
+            o = c.up(np.zeros((b["rows"], 16 * D), np.float16))
+            calls.append(({"cache": c.c, "batch": b, "q": c.rows(q, False), "o": o, "Hq": 16}, o))
+            own.kv_attention(calls[-1][0])
+        want = [own.read(o, np.uint16) for _, o in calls]
+        own.graph_begin()
+        own.kv_attention(calls[0][0])
+        g = own.graph_end()
+        for _ in range(4):
+            for (_, o), w in zip(calls, want):
+                own.upload(np.zeros_like(w), o)
+            dev.graph_launch(g)
+            own.kv_attention(calls[1][0])
+            dev.graph_launch(g)
+            dev.done()
+            for (_, o), w in zip(calls, want):
+                np.testing.assert_array_equal(own.read(o, np.uint16), w)
+        c.free()
+        own.close()
+        with pytest.raises(p0k.P0kError, match="destroyed"):
+            dev.graph_launch(g)
+    finally:
+        own.close()
+        if g is not None:
+            dev.graph_destroy(g)
+
+
+@pytest.mark.gpu
 def test_prompt_then_gemm_heads(dev):
     """the cache takes Q, K, V as the gemm's `heads` epilogue lays them out, and the attention's rows go on as gemm input"""
     from cases import make_case
