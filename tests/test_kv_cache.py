@@ -881,6 +881,51 @@ def test_graph_through_another_context(dev, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 90, 400])
+def test_layers_in_one_buffer(dev, n):
+    """two layers' caches behind offsets of the same buffers, with one page table behind an offset too, and Q, K, V as parts of
+    the same rows ([row][Hq + 2 Hkv][128]); the attention's rows into a part of wider ones"""
+    rng = np.random.default_rng(34)
+    L, Hq, Hkv, pages, mp = p0k.lib(), 6, 2, 14, 13
+    bufs = []
+
+    def up(x):
+        bufs.append(dev.upload(np.ascontiguousarray(x)))
+        return bufs[-1]
+    size = {"code": L.p0k_kv_code_bytes(pages, Hkv), "scale": L.p0k_kv_scale_bytes(pages, Hkv), "tail": L.p0k_kv_tail_bytes(1, Hkv)}
+    mem = {k: up(np.zeros(32 + 2 * v, np.uint8)) for k, v in size.items()}
+    table = up(np.concatenate([[7], rng.permutation(pages)[:mp]]).astype(np.int32))
+    layers = [{**{k: {"buf": mem[k], "off": 16 + i * size[k]} for k in size}, "table": {"buf": table, "off": 4}, "pages": pages, "slots": 1,
+               "max_pages": mp, "Hkv": Hkv} for i in range(2)]
+    W = Hq + 2 * Hkv
+    st = {"rs": W * D, "hs": D}
+    try:
+        refs = [Ref(1, Hkv) for _ in layers]
+        for p, m in ((0, 333), (333, n)):
+            b = {"pos": up(np.array([p], np.int32)), "cu": up(np.array([0, m], np.int32)), "B": 1, "rows": m}
+            for c, ref in zip(layers, refs):
+                x = rng.standard_normal((m, W, D)).astype(np.float16)
+                row = up(x)
+                dev.kv_append({"cache": c, "batch": b, "k": {"buf": row, "off": Hq * 256, **st}, "v": {"buf": row, "off": (Hq + Hkv) * 256, **st}})
+                ref.append(0, p, x[:, Hq:Hq + Hkv], x[:, Hq + Hkv:])
+                ref.last = x, row
+        for c, ref in zip(layers, refs):
+            x, row = ref.last
+            o = up(np.full((n, 8 * D), 0x1234, np.uint16))
+            dev.kv_attention({"cache": c, "batch": b, "q": {"buf": row, **st}, "o": {"buf": o, "off": D * 2, "ld": 8 * D}, "Hq": Hq})
+            got = dev.read(o, np.uint16, n * 8 * D).reshape(n, 8, D)
+            assert np.all(got[:, 0] == 0x1234) and np.all(got[:, 7] == 0x1234)
+            w, tol = attend_ref(x[:, :Hq], 333, *ref.held(0, read=False), Hq // Hkv)
+            assert np.all(np.abs(got[:, 1:7].copy().view(np.float16).astype(np.float64) - w) <= tol)
+        for k in size:
+            assert np.all(dev.read(mem[k], np.uint8, 16) == 0) and np.all(dev.read(mem[k], np.uint8, 16, 16 + 2 * size[k]) == 0)
+    finally:
+        dev.done()
+        for x in bufs:
+            dev.free(x)
+
+
+@pytest.mark.gpu
 def test_prompt_then_gemm_heads(dev):
     """the cache takes Q, K, V as the gemm's `heads` epilogue lays them out, and the attention's rows go on as gemm input"""
     from cases import make_case
