@@ -174,17 +174,21 @@ typedef struct p0k_batch {
 
 /* p0k_kv_cache: keys and values of `slots` sequences, in blocks of 64 tokens. A whole block lies in a page of the pool:
  * int8 codes of each kv head's 64 x 128 keys and values with one fp32 scale each (value = code * scale). Block k of
- * sequence s is page table[s][k] (int32). The block that a sequence is still filling and the one before it are held in
- * f16 in its tail. Buffers: p0k_kv_code_bytes / p0k_kv_scale_bytes / p0k_kv_tail_bytes; their inner layout is the
- * library's. Pages of whole blocks may be shared by sequences, as long as none of them goes back into such a block. A table
- * entry outside [0, pages): the block is not there (not written, not seen, read back as zeros). The page of a block is written
- * when the block becomes whole; until then its entry may stay unset. */
+ * sequence s is page table[s][k] (int32). A sequence's tail has two places for blocks in f16, k % 2: the block that it is
+ * still filling is in one, and in the other the one before it, unless a later block took that place before the sequence went
+ * back. `held` (optional) says which block each place holds, so that a sequence may go back to any of its tokens (see
+ * p0k_kv_append). Buffers: p0k_kv_code_bytes / p0k_kv_scale_bytes / p0k_kv_tail_bytes / p0k_kv_held_bytes; their inner layout
+ * is the library's, `held` begins as zeros (as p0k_alloc gives it). Pages of whole blocks may be shared by sequences, as long
+ * as none of them goes back into such a block. A table entry outside [0, pages): the block is not there (not written, not
+ * seen, read back as zeros). The page of a block is written when the block becomes whole; until then its entry may stay
+ * unset. */
 typedef struct p0k_kv_cache {
   void *code_buf; uint64_t code_off, code_size;           /* codes, tail: 16-byte aligned; scales: 8-byte */
   float *scale_buf; uint64_t scale_off, scale_size;
   void *tail_buf; uint64_t tail_off, tail_size;
   const int32_t *table_buf; uint64_t table_off, table_size;   /* [slots][max_pages] */
   uint32_t pages, slots, max_pages, Hkv;
+  int32_t *held_buf; uint64_t held_off, held_size;        /* optional */
 } p0k_kv_cache;
 
 /* rotary positions: y = x rotated by the angles a_i = t f_i of its token t, i < rd / 2: pairs (2 i, 2 i + 1) or, mode
@@ -212,8 +216,14 @@ typedef struct p0k_rope_args {
 /* kv_append: rows of K and V [Hkv] into the cache as tokens pos[b] .. of sequence b. Values are held to +-65504, NaN counts
  * as 0. A block that becomes whole is quantised from the f16 values of all of its tokens: scale = max |x| / 127 in fp32 (1
  * where all are 0), code = x / scale rounded to the nearest, ties to even. So the cache depends on the tokens only, not on
- * how many came with a call. A sequence may go back: pos may be any place from the start of the block before the one that
- * was being filled (64 tokens back or more; rejected draft tokens). Tokens from max_pages * 64 on are not kept. */
+ * how many came with a call. Tokens from max_pages * 64 on are not kept.
+ * A sequence may go back (rejected draft tokens): pos may be any place up to its end, but not before the token at which it
+ * began in this slot. A call that starts inside a block needs the block's earlier tokens in f16. The tail has them until
+ * a token of another block of the same k % 2 is written: always when a sequence goes back no further than to the start of the
+ * block before the furthest one that it has written in. Where the tail has them no more, and the cache has `held`, they
+ * become what p0k_kv_read gave for them before the call (zeros where the block has no page), and go on from there; without
+ * `held` such a call is not allowed, as nothing tells it from others (start it at the block's first token instead: that is
+ * right for any block). */
 typedef struct p0k_kv_append_args {
   uint32_t struct_size;
   p0k_kv_cache cache;
@@ -338,6 +348,7 @@ int p0k_rope(p0k_ctx *ctx, const p0k_rope_args *a);
 uint64_t p0k_kv_code_bytes(uint32_t pages, uint32_t Hkv);
 uint64_t p0k_kv_scale_bytes(uint32_t pages, uint32_t Hkv);
 uint64_t p0k_kv_tail_bytes(uint32_t slots, uint32_t Hkv);
+uint64_t p0k_kv_held_bytes(uint32_t slots, uint32_t Hkv);
 int p0k_kv_append_check(const p0k_kv_append_args *a);
 int p0k_kv_append(p0k_ctx *ctx, const p0k_kv_append_args *a);
 int p0k_kv_read_check(const p0k_kv_read_args *a);

@@ -94,6 +94,10 @@ static int check_cache(std::string *err, const char *op, const p0k_kv_cache &c, 
   o->scales = c.scale_buf + c.scale_off / 4;
   o->tail = (uint16_t *)((uint8_t *)c.tail_buf + c.tail_off);
   o->table = c.table_buf + c.table_off / 4;
+  if (c.held_buf) {
+    CHECK(check_ints(err, op, "held", c.held_buf, c.held_off, c.held_size, p0k_kv_held_bytes(c.slots, c.Hkv) / 4));
+    o->held = c.held_buf + c.held_off / 4;
+  }
   o->pages = c.pages; o->slots = c.slots; o->max_pages = c.max_pages; o->Hkv = c.Hkv;
   return P0K_OK;
 }
@@ -211,4 +215,5 @@ extern "C" {
 uint64_t p0k_kv_code_bytes(uint32_t pages, uint32_t Hkv) { return (uint64_t)pages * Hkv * 2 * p0k::KV_HEAD; }
 uint64_t p0k_kv_scale_bytes(uint32_t pages, uint32_t Hkv) { return (uint64_t)pages * Hkv * 8; }
 uint64_t p0k_kv_tail_bytes(uint32_t slots, uint32_t Hkv) { return (uint64_t)slots * Hkv * 8 * p0k::KV_HEAD; }
+uint64_t p0k_kv_held_bytes(uint32_t slots, uint32_t Hkv) { return (uint64_t)slots * Hkv * 16; }
 }

@@ -9,7 +9,7 @@
 //   values  16-byte pieces of 8 tokens of d and of d + 16:     [half of 32 tokens][32 d][token group][d % 16]
 // where token group q of a half holds its tokens 4 q .. 4 q + 3 and 16 + 4 q .. + 3: the eight tokens of which a lane of the
 // 16x16x32 product K Q^T holds the scores (and, groups q and q + 2, those of a lane of the 32x32x16 product).
-// A sequence's tail holds two blocks (k % 2) in f16, in the same order with pieces of 8 values:
+// A sequence's tail has places for two blocks (k % 2) in f16, in the same order with pieces of 8 values:
 //   keys    [half][16-token tile][32 d's two steps of 8: 64 d, 8 d][16 d][token % 16]      values  [half][16 d][group][d % 16]
 #pragma once
 #include <hip/hip_runtime.h>
@@ -26,6 +26,7 @@ struct KvParams {
   float *scales;           // [pages][Hkv][K, V]
   uint16_t *tail;          // [slots][2][Hkv][K, V][KV_HEAD] f16
   const int32_t *table;    // [slots][max_pages]
+  int32_t *held;           // [slots][Hkv][K, V][2]: 1 + the block that the tail's place holds, 0: none (null: not kept)
   uint32_t pages, slots, max_pages, Hkv;
   const int32_t *pos, *cu, *slot, *len;   // slot, len may be null
   uint32_t B, rows;
@@ -125,6 +126,9 @@ __device__ __forceinline__ uint64_t kv_scale_at(const KvParams &p, uint32_t page
 }
 __device__ __forceinline__ uint64_t kv_tail_at(const KvParams &p, uint32_t slot, uint32_t block, uint32_t h, uint32_t kv) {
   return ((((uint64_t)slot * 2 + (block & 1)) * p.Hkv + h) * 2 + kv) * KV_HEAD;
+}
+__device__ __forceinline__ int32_t *kv_held(const KvParams &p, uint32_t slot, uint32_t h, uint32_t kv) {
+  return p.held + (((uint64_t)slot * p.Hkv + h) * 2 + kv) * 2;
 }
 // page of a block of a slot: 0xffffffff where there is none
 __device__ __forceinline__ uint32_t kv_page(const KvParams &p, uint32_t slot, uint32_t block) {

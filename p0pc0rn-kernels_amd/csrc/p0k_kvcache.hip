@@ -140,13 +140,51 @@ struct Part {
 // reads at once lie at the same places of 16 runs
 __device__ __forceinline__ uint32_t kv_lds(uint32_t code) { return code + (code >> 8) * 16; }
 
+// code * scale of byte j of a word (byte = code + 128; 128 s is exact, so the fma rounds code * s once)
+__device__ __forceinline__ uint16_t kv_value(uint32_t w, int j, float sc) {
+  float v = fmaf((float)((w >> (8 * j)) & 255u), sc, -128.0f * sc);
+  asm volatile("" : "+v"(v));                     // (rounded to fp32 before it is rounded to f16)
+  return __builtin_bit_cast(uint16_t, (f16)v);
+}
+
+// a block's values x from its codes, as f16, those whose token passes `is` (by the whole workgroup; values go through LDS)
+template <int KV, class F>
+__device__ __forceinline__ void load_codes(const KvParams &p, const Part<KV> &part, uint32_t page, uint32_t h, u16x8 *x, uint8_t *sC, F is) {
+  const uint8_t *codes = p.codes + kv_code_at(p, page, h, KV);
+  const float sc = p.scales[kv_scale_at(p, page, h, KV)];
+  if constexpr (KV == 0) {
+    if (!is(part.tok(0))) return;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const u32x4 w = *(const u32x4 *)(codes + kv_kcode(part.tok(0), part.d(2 * i)));
+#pragma unroll
+      for (int j = 0; j < 16; j++) x[2 * i + (j >> 3)][j & 7] = kv_value(w[j >> 2], j & 3, sc);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; i++) *(u32x4 *)(sC + kv_lds(16 * (part.tid + 256 * i))) = *(const u32x4 *)(codes + 16 * (part.tid + 256 * i));
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const uint32_t w = *(const uint32_t *)(sC + kv_lds(kv_vcode(part.tok(0), part.d(0) + j)));
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (is(part.tok(i))) x[i][j] = kv_value(w, i, sc);
+    }
+  }
+}
+
 template <int KV>
 __device__ void append_block(const KvParams &p, const KvSeq &s, uint32_t blk, uint32_t k0, uint32_t end, uint32_t h, uint8_t *sC, float *sMax) {
   const uint32_t tid = threadIdx.x;
   const Part<KV> part{tid};
   const uint16_t *X = (KV ? p.V : p.K) + (KV ? p.vhs : p.khs) * h;
   const uint64_t rs = KV ? p.vrs : p.krs;
-  const uint32_t page = kv_page(p, s.slot, blk);
+  const int32_t entry = p.table[(uint64_t)s.slot * p.max_pages + blk];   // (asked for before it is needed)
+  auto page_of = [&] { return entry >= 0 && (uint32_t)entry < p.pages ? (uint32_t)entry : 0xffffffffu; };
+  const bool inside = blk * KV_T < s.pos;
+  int32_t *held = p.held && blk == k0 ? kv_held(p, s.slot, h, KV) : nullptr;
+  const int32_t places = held ? held[tid & 1] : 0;
   u16x8 x[4];
   // the values of a block that this call brings
   auto fresh = [&](uint32_t block) {
@@ -157,10 +195,10 @@ __device__ void append_block(const KvParams &p, const KvSeq &s, uint32_t blk, ui
     }
     kv_hold(x);
   };
-  auto keep = [&](uint32_t block) {              // and into the tail
+  auto keep = [&](uint32_t block, uint32_t from, uint32_t to) {   // and into the tail, the tokens from .. to - 1
     part.store_tail(p.tail + kv_tail_at(p, s.slot, block, h, KV), x, [&](uint32_t t) {
       const uint32_t tt = block * KV_T + t;
-      return tt >= s.pos && tt < end;
+      return tt >= from && tt < to;
     });
   };
 #pragma unroll
@@ -169,9 +207,23 @@ __device__ void append_block(const KvParams &p, const KvSeq &s, uint32_t blk, ui
   // The tail keeps the last block and the one before it. Of its two places, the first block's may still be read (the tokens
   // that it held before this call): that block's workgroup writes it, after it has read.
   const uint32_t last = end / KV_T;
-  if (blk + 1 >= last && (blk == k0 || ((blk ^ k0) & 1))) keep(blk);
+  const bool kept = blk + 1 >= last && (blk == k0 || ((blk ^ k0) & 1));
+  if (kept) keep(blk, s.pos, end);
+  // lost: the block's tokens before this call's are no longer in the tail in f16; the codes' values take their place
+  const int32_t held0 = (int32_t)__builtin_amdgcn_readlane(places, 0), held1 = (int32_t)__builtin_amdgcn_readlane(places, 1);
+  const bool lost = held && inside && (blk & 1 ? held1 : held0) != (int32_t)blk + 1;
+  if (__builtin_expect(lost, 0)) {
+    const uint32_t page = page_of();
+    if (page != 0xffffffffu) {
+      load_codes(p, part, page, h, x, sC, [&](uint32_t t) { return blk * KV_T + t < s.pos; });
+      kv_hold(x);                                // (a page that no call has written)
+    }
+    if (kept) keep(blk, 0, s.pos);
+  }
   if ((blk + 1) * KV_T <= end) {
-    if (blk * KV_T < s.pos) {
+    const uint32_t page = page_of();
+    const bool have = page != 0xffffffffu;
+    if (inside && !lost) {
       part.load_tail(p.tail + kv_tail_at(p, s.slot, blk, h, KV), x, sC, [&](uint32_t t) { return blk * KV_T + t < s.pos; });
       kv_hold(x);                                // (a tail that no call has written)
     }
@@ -181,7 +233,6 @@ __device__ void append_block(const KvParams &p, const KvSeq &s, uint32_t blk, ui
     __syncthreads();
     const float amax = fmaxf(fmaxf(sMax[0], sMax[1]), fmaxf(sMax[2], sMax[3]));
     const float sc = amax > 0.0f ? amax / 127.0f : 1.0f;
-    const bool have = page != 0xffffffffu;
     uint8_t *codes = p.codes + kv_code_at(p, have ? page : 0u, h, KV);
     uint32_t w[8];
     kv_codes<KV>(x, sc, w);
@@ -205,7 +256,24 @@ __device__ void append_block(const KvParams &p, const KvSeq &s, uint32_t blk, ui
     if (last >= 1 && cb > k0 && cb * KV_T < end) {
       __syncthreads();                           // (the whole workgroup has read the first block's tokens)
       fresh(cb);
-      keep(cb);
+      keep(cb, s.pos, end);
+    }
+    if (held) {
+      // What the places hold now: the last block and the one before it where this call brought tokens of theirs; no block
+      // that this call wrote otherwise, and none that it left behind by going back. (Mostly as it was: nothing to write.)
+      auto now = [&](uint32_t q, int32_t was) {
+        const uint32_t b = ((last ^ q) & 1) ? last - 1 : last;     // the one of the last two in place q
+        if ((last >= 1 || q == 0) && b >= k0 && b * KV_T < end) return (int32_t)b + 1;
+        return was > (int32_t)k0 ? 0 : was;
+      };
+      const int32_t n0 = now(0, held0), n1 = now(1, held1);
+      if (__any(n0 != held0 || n1 != held1)) {
+        __syncthreads();                         // (the whole workgroup has read them)
+        if (tid == 0) {
+          held[0] = n0;
+          held[1] = n1;
+        }
+      }
     }
   }
 }
@@ -224,13 +292,6 @@ __global__ __launch_bounds__(256, 8) void k_kv_append(KvParams p) {
   else append_block<1>(p, s, blk, k0, end, h, sC, sMax);
 }
 
-// code * scale of byte j of a word (byte = code + 128; 128 s is exact, so the fma rounds code * s once)
-__device__ __forceinline__ uint16_t kv_value(uint32_t w, int j, float sc) {
-  float v = fmaf((float)((w >> (8 * j)) & 255u), sc, -128.0f * sc);
-  asm volatile("" : "+v"(v));                     // (rounded to fp32 before it is rounded to f16)
-  return __builtin_bit_cast(uint16_t, (f16)v);
-}
-
 template <int KV>
 __device__ void read_block(const KvParams &p, const KvSeq &s, uint32_t blk, uint32_t len, uint32_t h, uint8_t *sC) {
   const uint32_t tid = threadIdx.x, end = s.pos + s.n;
@@ -242,26 +303,7 @@ __device__ void read_block(const KvParams &p, const KvSeq &s, uint32_t blk, uint
   if (blk == len / KV_T) {
     part.load_tail(p.tail + kv_tail_at(p, s.slot, blk, h, KV), x, sC, [&](uint32_t t) { return blk * KV_T + t < len; });
   } else if (page != 0xffffffffu) {
-    const uint8_t *codes = p.codes + kv_code_at(p, page, h, KV);
-    const float sc = p.scales[kv_scale_at(p, page, h, KV)];
-    if constexpr (KV == 0) {
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const u32x4 w = *(const u32x4 *)(codes + kv_kcode(part.tok(0), part.d(2 * i)));
-#pragma unroll
-        for (int j = 0; j < 16; j++) x[2 * i + (j >> 3)][j & 7] = kv_value(w[j >> 2], j & 3, sc);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; i++) *(u32x4 *)(sC + kv_lds(16 * (tid + 256 * i))) = *(const u32x4 *)(codes + 16 * (tid + 256 * i));
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const uint32_t w = *(const uint32_t *)(sC + kv_lds(kv_vcode(part.tok(0), part.d(0) + j)));
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[i][j] = kv_value(w, i, sc);
-      }
-    }
+    load_codes(p, part, page, h, x, sC, [](uint32_t) { return true; });
   }
   uint16_t *Y = (KV ? p.Vo : p.Ko) + (KV ? p.vhs : p.khs) * h;
 #pragma unroll

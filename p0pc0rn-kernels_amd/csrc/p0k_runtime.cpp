@@ -915,7 +915,7 @@ static int check_live_cache(p0k_ctx *c, const p0k_kv_cache &k, const char *op) {
   if ((r = check_live(c, k.code_buf, k.code_size, op, "code")) || (r = check_live(c, k.scale_buf, k.scale_size, op, "scale")) ||
       (r = check_live(c, k.tail_buf, k.tail_size, op, "tail")) || (r = check_live(c, k.table_buf, k.table_size, op, "table")))
     return r;
-  return P0K_OK;
+  return k.held_buf ? check_live(c, k.held_buf, k.held_size, op, "held") : P0K_OK;
 }
 
 int p0k_rope_check(const p0k_rope_args *a) {

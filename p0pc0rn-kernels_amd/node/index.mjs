@@ -270,7 +270,7 @@ function batchDesc(d, b) {
 }
 function cacheDesc(a) {
   const d = { pages: a.cache.pages, slots: a.cache.slots, max_pages: a.cache.maxPages, Hkv: a.cache.Hkv };
-  for (const n of ['code', 'scale', 'tail', 'table']) operand(d, n, a.cache[n]);
+  for (const n of ['code', 'scale', 'tail', 'table', 'held']) operand(d, n, a.cache[n]);
   batchDesc(d, a.batch);
   return d;
 }
@@ -290,11 +290,11 @@ function rope(gpu, a) {
 /** kvCache(gpu, {Hkv, pages, slots, maxPages, table}): the buffers of a cache, `pages` pages of 64 tokens for `slots` sequences of
  *  up to maxPages blocks. table: Int32 [slots][maxPages] buffer of page numbers (default: sequence s owns pages s * maxPages on) */
 function kvCache(gpu, o) {
-  const [code, scale, tail] = call(addon().kvBytes, o.pages, o.slots, o.Hkv);
+  const [code, scale, tail, held] = call(addon().kvBytes, o.pages, o.slots, o.Hkv);
   let table = o.table;
   if (!table) table = gpu.upload(Int32Array.from({ length: o.slots * o.maxPages }, (_, i) => (i < o.pages ? i : -1)), 'kv table');
-  return { code: gpu.buffer(code, 'kv codes'), scale: gpu.buffer(scale, 'kv scales'), tail: gpu.buffer(tail, 'kv tail'), table,
-    pages: o.pages, slots: o.slots, maxPages: o.maxPages, Hkv: o.Hkv };
+  return { code: gpu.buffer(code, 'kv codes'), scale: gpu.buffer(scale, 'kv scales'), tail: gpu.buffer(tail, 'kv tail'),
+    held: gpu.buffer(held, 'kv held'), table, pages: o.pages, slots: o.slots, maxPages: o.maxPages, Hkv: o.Hkv };
 }
 
 /** kvAppend(gpu, {cache, batch, k, v}): rows of K / V into the cache */

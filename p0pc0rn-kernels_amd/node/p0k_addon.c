@@ -464,7 +464,7 @@ static int batch_of(napi_env env, napi_value o, p0k_batch *b) {
          fields_u32(env, o, (const char *const[]){"B", "rows"}, (uint32_t *const[]){&b->B, &b->rows}, 2);
 }
 static int cache_of(napi_env env, napi_value o, p0k_kv_cache *c) {
-  return OPERAND(o, code, *c) && OPERAND(o, scale, *c) && OPERAND(o, tail, *c) && OPERAND(o, table, *c) &&
+  return OPERAND(o, code, *c) && OPERAND(o, scale, *c) && OPERAND(o, tail, *c) && OPERAND(o, table, *c) && OPERAND(o, held, *c) &&
          fields_u32(env, o, (const char *const[]){"pages", "slots", "max_pages", "Hkv"},
                     (uint32_t *const[]){&c->pages, &c->slots, &c->max_pages, &c->Hkv}, 4);
 }
@@ -497,16 +497,17 @@ static napi_value rope(napi_env env, napi_callback_info info) {   /* (ctx, desc,
   return r ? throw_p0k(env, r) : undef(env);
 }
 
-static napi_value kvBytes(napi_env env, napi_callback_info info) {   /* (pages, slots, Hkv) -> [codes, scales, tail] */
+static napi_value kvBytes(napi_env env, napi_callback_info info) {   /* (pages, slots, Hkv) -> [codes, scales, tail, held] */
   napi_value argv[3], out;
   uint64_t v[3];
   if (!get_args(env, info, 3, argv)) return NULL;
   for (int i = 0; i < 3; i++)
     if (!to_u64(env, argv[i], &v[i]) || v[i] > 0xffffffffu) { napi_throw_type_error(env, NULL, "pages, slots, Hkv"); return NULL; }
-  CHECK_NAPI(env, napi_create_array_with_length(env, 3, &out));
+  CHECK_NAPI(env, napi_create_array_with_length(env, 4, &out));
   CHECK_NAPI(env, napi_set_element(env, out, 0, mk_num(env, (double)p0k_kv_code_bytes((uint32_t)v[0], (uint32_t)v[2]))));
   CHECK_NAPI(env, napi_set_element(env, out, 1, mk_num(env, (double)p0k_kv_scale_bytes((uint32_t)v[0], (uint32_t)v[2]))));
   CHECK_NAPI(env, napi_set_element(env, out, 2, mk_num(env, (double)p0k_kv_tail_bytes((uint32_t)v[1], (uint32_t)v[2]))));
+  CHECK_NAPI(env, napi_set_element(env, out, 3, mk_num(env, (double)p0k_kv_held_bytes((uint32_t)v[1], (uint32_t)v[2]))));
   return out;
 }
 

@@ -126,7 +126,7 @@ class Batch(C.Structure):
 
 class KvCache(C.Structure):
     _fields_ = (_operand("code") + _operand("scale") + _operand("tail") + _operand("table") +
-                [(n, C.c_uint32) for n in ("pages", "slots", "max_pages", "Hkv")])
+                [(n, C.c_uint32) for n in ("pages", "slots", "max_pages", "Hkv")] + _operand("held"))
 
 
 class RopeArgs(C.Structure):
@@ -179,6 +179,8 @@ def _set_batch(s, b, resolve):
 def _set_cache(s, c, resolve):
     for n in ("code", "scale", "tail", "table"):
         _set_operand(s, n, c[n], resolve)
+    if c.get("held") is not None:
+        _set_operand(s, "held", c["held"], resolve)
     s.pages, s.slots, s.max_pages, s.Hkv = c["pages"], c["slots"], c["max_pages"], c["Hkv"]
 
 
@@ -264,7 +266,7 @@ EXPORTS = [
     "p0k_free", "p0k_drain_pool", "p0k_pool_stats_get", "p0k_upload", "p0k_download", "p0k_copy", "p0k_sync",
     "p0k_gemm_check", "p0k_gemm", "p0k_gemm_flops", "p0k_select_tile", "p0k_rowstats_check", "p0k_rowstats",
     "p0k_attention_check", "p0k_attention", "p0k_attention_flops",
-    "p0k_rope_check", "p0k_rope", "p0k_kv_code_bytes", "p0k_kv_scale_bytes", "p0k_kv_tail_bytes",
+    "p0k_rope_check", "p0k_rope", "p0k_kv_code_bytes", "p0k_kv_scale_bytes", "p0k_kv_tail_bytes", "p0k_kv_held_bytes",
     "p0k_kv_append_check", "p0k_kv_append", "p0k_kv_read_check", "p0k_kv_read", "p0k_kv_attention_check", "p0k_kv_attention",
     "p0k_pixstats", "p0k_gn_part_bytes", "p0k_gn_partial", "p0k_gn_finalize", "p0k_groupnorm_stats",
     "p0k_event_create", "p0k_event_record", "p0k_event_elapsed_ms", "p0k_event_destroy",
@@ -305,7 +307,7 @@ def lib():
             "p0k_attention_flops": ([C.POINTER(AttnArgs)], C.c_double),
             "p0k_rope_check": ([C.POINTER(RopeArgs)], I), "p0k_rope": ([P, C.POINTER(RopeArgs)], I),
             "p0k_kv_code_bytes": ([C.c_uint32, C.c_uint32], U64), "p0k_kv_scale_bytes": ([C.c_uint32, C.c_uint32], U64),
-            "p0k_kv_tail_bytes": ([C.c_uint32, C.c_uint32], U64),
+            "p0k_kv_tail_bytes": ([C.c_uint32, C.c_uint32], U64), "p0k_kv_held_bytes": ([C.c_uint32, C.c_uint32], U64),
             "p0k_kv_append_check": ([C.POINTER(KvAppendArgs)], I), "p0k_kv_append": ([P, C.POINTER(KvAppendArgs)], I),
             "p0k_kv_read_check": ([C.POINTER(KvReadArgs)], I), "p0k_kv_read": ([P, C.POINTER(KvReadArgs)], I),
             "p0k_kv_attention_check": ([C.POINTER(KvAttnArgs)], I), "p0k_kv_attention": ([P, C.POINTER(KvAttnArgs)], I),
@@ -562,7 +564,8 @@ class Device:
     def kv_cache(self, Hkv, pages, slots, max_pages, table=None):
         """The buffers of an 8-bit key / value cache (p0k_kv_cache of p0k.h) as the `cache` of the kv_* calls: `pages` pages of
         64 tokens for all kv heads, `slots` sequences of up to max_pages blocks. table: int32 [slots][max_pages] page
-        numbers, -1 where there is none; without one, sequence s owns pages s * max_pages on."""
+        numbers, -1 where there is none; without one, sequence s owns pages s * max_pages on. `held` lets sequences go
+        back to any of their tokens."""
         L, own = lib(), table is None
         if own:
             t = np.full((slots, max_pages), -1, np.int32)
@@ -570,13 +573,13 @@ class Device:
             t.reshape(-1)[:n] = np.arange(n)
             table = self.upload(t)
         return {"code": self.buffer(L.p0k_kv_code_bytes(pages, Hkv)), "scale": self.buffer(L.p0k_kv_scale_bytes(pages, Hkv)),
-                "tail": self.buffer(L.p0k_kv_tail_bytes(slots, Hkv)), "table": table,
+                "tail": self.buffer(L.p0k_kv_tail_bytes(slots, Hkv)), "held": self.buffer(L.p0k_kv_held_bytes(slots, Hkv)), "table": table,
                 "pages": pages, "slots": slots, "max_pages": max_pages, "Hkv": Hkv, "own_table": own}
 
     def kv_cache_free(self, cache):
         """gives the cache's buffers back (a table that came from the caller stays the caller's)"""
-        for n in ("code", "scale", "tail") + (("table",) if cache["own_table"] else ()):
-            self.free(cache[n])
+        for n in ("code", "scale", "tail", "held") + (("table",) if cache["own_table"] else ()):
+            self.free(cache.get(n))
 
     def kv_append_raw(self, s):
         _chk(lib().p0k_kv_append(self.ctx, C.byref(s)))
