@@ -806,8 +806,13 @@ __global__ __launch_bounds__(64 * NW, 2) void k_kv_attn_block(KvParams p, uint32
                                                 pack_o(oacc[db][4 * g4 + 2] * inv, oacc[db][4 * g4 + 3] * inv)};
 }
 
-// The runs of k_kv_attn_block together: a half wave for a row of a head, four d a thread
+// The runs of k_kv_attn_block together: a half wave for a row of a head, four d a thread. With offsets that decrease not every
+// row has parts, and two sequences may have left theirs in the same place: nothing to join then. (B is small here: the blocks of
+// all sequences and heads are fewer than two a CU.)
 __global__ __launch_bounds__(256) void k_kv_attn_join(KvParams p, uint32_t S, const float *part) {
+  bool down = false;
+  for (uint32_t b = threadIdx.x; b < p.B; b += 256) down |= kv_row0(p.cu, b + 1, p.rows) < kv_row0(p.cu, b, p.rows);
+  if (__syncthreads_or(down)) return;
   const uint64_t it = (uint64_t)blockIdx.x * 256 + threadIdx.x, rh = it >> 5, n = (uint64_t)p.rows * p.Hq;
   if (rh >= n) return;
   const uint32_t r = (uint32_t)(rh / p.Hq), h = (uint32_t)(rh - (uint64_t)r * p.Hq), d = 4 * ((uint32_t)it & 31u);
