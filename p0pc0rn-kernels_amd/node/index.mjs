@@ -275,11 +275,15 @@ function cacheDesc(a) {
   return d;
 }
 
-/** rope(gpu, {x, y (default x: in place), H, batch, rd, mode: 'interleaved' | 'half', theta, scaling: {kind: 'linear' | 'bands',
- *  factor, orig, low, high}, freqs, mscale}): rotary positions */
+const ROPE_MODE = { __proto__: null, interleaved: 0, half: 1 }, ROPE_SCALING = { __proto__: null, plain: 0, linear: 1, bands: 2 };
+/** rope(gpu, {x, y (default x: in place), H, batch, rd, mode: 'interleaved' | 'half', theta, scaling: {kind: 'plain' | 'linear' |
+ *  'bands', factor, orig, low, high}, freqs, mscale}): rotary positions */
 function rope(gpu, a) {
-  const sc = a.scaling || {};
-  const d = { H: a.H, rd: a.rd || 0, mode: a.mode === 'half' ? 1 : 0, scaling: { linear: 1, bands: 2 }[sc.kind] || 0, theta: a.theta || 0,
+  const sc = a.scaling || { kind: 'plain' };
+  const mode = ROPE_MODE[a.mode || 'interleaved'], scaling = ROPE_SCALING[sc.kind];
+  if (mode === undefined) throw new Error(`rope: unknown mode ${a.mode}`);
+  if (scaling === undefined) throw new Error(`rope: unknown scaling kind ${sc.kind}`);
+  const d = { H: a.H, rd: a.rd || 0, mode, scaling, theta: a.theta || 0,
     factor: sc.factor || 0, orig: sc.orig || 0, low: sc.low || 0, high: sc.high || 0, mscale: a.mscale || 0 };
   operand(d, 'x', a.x);
   operand(d, 'y', a.y || a.x);
