@@ -233,7 +233,8 @@ typedef struct p0k_kv_append_args {
 } p0k_kv_append_args;
 
 /* kv_read: row r of K and V = the cached token pos[b] + r - cu[b] of sequence b, in f16 (code * scale rounded once; the
- * open block's values as they are), zeros where there is none. len[b] (int32 [B]): tokens that sequence b holds. */
+ * open block's values as they are), zeros where there is none. len[b] (int32 [B]): tokens that sequence b holds. k and v must not
+ * overlap. */
 typedef struct p0k_kv_read_args {
   uint32_t struct_size;
   p0k_kv_cache cache;
@@ -246,7 +247,7 @@ typedef struct p0k_kv_read_args {
 /* kv_attention: O [rows][ldo] f16, head h at column h * 128 = softmax(scale q.k) v over the cached tokens j that the query
  * at token t sees: j <= t and, with a window, j > t - window or j < sinks. The cache holds the batch's own rows already
  * (p0k_kv_append comes first): sequence b has pos[b] + cu[b + 1] - cu[b] tokens. Query head h reads kv head h / (Hq / Hkv).
- * A row that sees nothing is 0 (with offsets that decrease, rows may be left as they are). Zero fields: ldo = Hq * 128,
+ * A row that sees nothing is 0 (with offsets that decrease, rows may be left as they are). o and q must not overlap. Zero fields: ldo = Hq * 128,
  * scale = 1 / sqrt(128), window: none, cap: none (cap * tanh(s / cap) otherwise); scale in [2^-40, 2^40], cap in [2^-20,
  * 2^20]. o: 8-byte aligned, ldo a multiple of 4. Pages wholly outside every row's window are not read. The keys are divided
  * over workgroups through workspaces of the context: a fixed one, and with many queries after a long cache the one of split

@@ -59,6 +59,35 @@ static int check_heads(std::string *err, const char *op, const char *what, const
   return fits(err, op, what, off, (*rs * (rows - 1) + *hs * (H - 1) + 128) * 2, size);
 }
 
+// Whether two operands share no value: value d of row r and head h lies rs r + hs h + d halves behind an operand's first one.
+// Operands whose ranges meet are told apart where their rows have the same stride (parts of the same rows, or of the same heads);
+// where they have not, they count as overlapping.
+struct RowsAt { const void *buf; uint64_t off, rs, hs; uint32_t rows, H; };
+static bool apart(RowsAt a, RowsAt b) {
+  typedef __int128 i128;
+  if (a.rows == 0 || a.H == 0 || b.rows == 0 || b.H == 0) return true;
+  if (a.rows == 1) a.rs = b.rs;
+  if (b.rows == 1) b.rs = a.rs;
+  if (a.H == 1) a.hs = b.hs;
+  if (b.H == 1) b.hs = a.hs;
+  const i128 rs = a.rs, wa = (i128)a.hs * (a.H - 1) + 128, wb = (i128)b.hs * (b.H - 1) + 128;   // from a row's first value to its last
+  const i128 d = ((i128)(uintptr_t)b.buf + b.off - (i128)(uintptr_t)a.buf - a.off) / 2;          // from a's first value to b's
+  if (d >= (i128)a.rs * (a.rows - 1) + wa || -d >= (i128)b.rs * (b.rows - 1) + wb) return true;
+  if (a.rs != b.rs) return false;
+  // a row of b is i rows on from one of a's: is there such an i with -below < at + rs i < above?
+  auto meets = [&](i128 at, i128 below, i128 above) {
+    const i128 lo = 1 - (i128)a.rows, hi = (i128)b.rows - 1;
+    i128 i = (-below - at) / rs - 1;
+    while (at + rs * i <= -below) i++;             // the first i above the lower bound
+    if (i < lo) i = lo;
+    return i <= hi && at + rs * i < above;
+  };
+  if (a.hs != b.hs) return !meets(d, wb, wa);
+  for (i128 h = 1 - (i128)a.H; h < (i128)b.H; h++)
+    if (meets(d + (i128)a.hs * h, 128, 128)) return false;
+  return true;
+}
+
 static int check_ints(std::string *err, const char *op, const char *what, const void *buf, uint64_t off, uint64_t size, uint64_t n) {
   NEED(buf != nullptr, "%s: missing %s buffer", op, what);
   NEED(off % 4 == 0, "%s: %s offset must be a multiple of 4 bytes", op, what);
@@ -126,6 +155,7 @@ int prepare_kv_read(const p0k_kv_read_args *a, KvParams *out, std::string *err) 
   CHECK(check_ints(err, "kv_read", "len", a->len_buf, a->len_off, a->len_size, o.B));
   CHECK(check_heads(err, "kv_read", "k", a->k_buf, a->k_off, a->k_size, a->k_rs, a->k_hs, o.rows, o.Hkv, true, &o.krs, &o.khs));
   CHECK(check_heads(err, "kv_read", "v", a->v_buf, a->v_off, a->v_size, a->v_rs, a->v_hs, o.rows, o.Hkv, true, &o.vrs, &o.vhs));
+  NEED(apart({a->k_buf, a->k_off, o.krs, o.khs, o.rows, o.Hkv}, {a->v_buf, a->v_off, o.vrs, o.vhs, o.rows, o.Hkv}), "kv_read: k and v overlap");
   o.len = a->len_buf + a->len_off / 4;
   o.Ko = (uint16_t *)((uint8_t *)a->k_buf + a->k_off);
   o.Vo = (uint16_t *)((uint8_t *)a->v_buf + a->v_off);
@@ -148,6 +178,8 @@ int prepare_kv_attention(const p0k_kv_attn_args *a, KvParams *out, std::string *
   NEED(a->o_off % 8 == 0 && o.ldo % 4 == 0 && o.ldo >= a->Hq * 128,
        "kv_attention: o offset 8-byte aligned, ldo a multiple of 4 covering Hq * 128");
   if (o.rows) CHECK(fits(err, "kv_attention", "o", a->o_off, ((uint64_t)(o.rows - 1) * o.ldo + a->Hq * 128) * 2, a->o_size));
+  // (other workgroups may still read a row's queries when its results are stored)
+  NEED(apart({a->q_buf, a->q_off, o.krs, o.khs, o.rows, a->Hq}, {a->o_buf, a->o_off, o.ldo, 128, o.rows, a->Hq}), "kv_attention: q and o overlap");
   // the kernels count (unit of 32 tokens, head, 16 rows) in 32 bits, and a launch has fewer than 2^32 threads
   NEED((unsigned __int128)a->cache.max_pages * 2 * o.Hkv * ((uint64_t)o.rows * (a->Hq / o.Hkv) / 16 + o.B) < (1ull << 32) &&
            (uint64_t)o.Hkv * ((uint64_t)o.rows * (a->Hq / o.Hkv) / 128 + o.B) < (1ull << 23),
@@ -177,6 +209,9 @@ int prepare_rope(const p0k_rope_args *a, RopeParams *out, std::string *err) {
   CHECK(check_heads(err, "rope", "x", a->x_buf, a->x_off, a->x_size, a->x_rs, a->x_hs, b.rows, a->H, false, &o.xrs, &o.xhs));
   CHECK(check_heads(err, "rope", "y", a->y_buf, a->y_off, a->y_size, a->y_rs, a->y_hs, b.rows, a->H, true, &o.yrs, &o.yhs));
   NEED(a->x_buf != a->y_buf || a->x_off != a->y_off || (o.xrs == o.yrs && o.xhs == o.yhs), "rope: in place, x and y need the same strides");
+  NEED((a->x_buf == a->y_buf && a->x_off == a->y_off) ||
+           apart({a->x_buf, a->x_off, o.xrs, o.xhs, b.rows, a->H}, {a->y_buf, a->y_off, o.yrs, o.yhs, b.rows, a->H}),
+       "rope: x and y overlap (in place they have the same offset and strides)");
   o.X = (const uint16_t *)((const uint8_t *)a->x_buf + a->x_off);
   o.Y = (uint16_t *)((uint8_t *)a->y_buf + a->y_off);
   o.rd = a->rd ? a->rd : 128;
