@@ -247,11 +247,13 @@ typedef struct p0k_kv_read_args {
 /* kv_attention: O [rows][ldo] f16, head h at column h * 128 = softmax(scale q.k) v over the cached tokens j that the query
  * at token t sees: j <= t and, with a window, j > t - window or j < sinks. The cache holds the batch's own rows already
  * (p0k_kv_append comes first): sequence b has pos[b] + cu[b + 1] - cu[b] tokens. Query head h reads kv head h / (Hq / Hkv).
- * A row that sees nothing is 0 (with offsets that decrease, rows may be left as they are). o and q must not overlap. Zero fields: ldo = Hq * 128,
- * scale = 1 / sqrt(128), window: none, cap: none (cap * tanh(s / cap) otherwise); scale in [2^-40, 2^40], cap in [2^-20,
- * 2^20]. o: 8-byte aligned, ldo a multiple of 4. Pages wholly outside every row's window are not read. The keys are divided
- * over workgroups through workspaces of the context: a fixed one, and with many queries after a long cache the one of split
- * prompts (in a capture only where it has grown to the size before; neither in a capture begun by the caller). */
+ * A row that sees nothing is 0 (with offsets that decrease, rows may be left as they are). o and q must not overlap. Zero
+ * fields: ldo = Hq * 128, scale = 1 / sqrt(128), window: none, cap: none (cap * tanh(s / cap) otherwise); scale in [2^-40,
+ * 2^40], cap in [2^-20, 2^20]. o: 8-byte aligned, ldo a multiple of 4. rows * Hq / 256 + B * Hkv is below 2^23 (or, with at
+ * most 256 rows of a kv head a sequence on average, (rows * Hq / 16 + B * Hkv) * max_pages below 2^31). Pages wholly outside
+ * every row's window are not read. The keys are divided over workgroups through workspaces of the context: a fixed one, and
+ * with many queries after a long cache the one of split prompts (in a capture only where it has grown to the size before;
+ * neither in a capture begun by the caller). */
 typedef struct p0k_kv_attn_args {
   uint32_t struct_size;
   p0k_kv_cache cache;

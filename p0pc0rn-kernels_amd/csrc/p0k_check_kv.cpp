@@ -180,13 +180,13 @@ int prepare_kv_attention(const p0k_kv_attn_args *a, KvParams *out, std::string *
   if (o.rows) CHECK(fits(err, "kv_attention", "o", a->o_off, ((uint64_t)(o.rows - 1) * o.ldo + a->Hq * 128) * 2, a->o_size));
   // (other workgroups may still read a row's queries when its results are stored)
   NEED(apart({a->q_buf, a->q_off, o.krs, o.khs, o.rows, a->Hq}, {a->o_buf, a->o_off, o.ldo, 128, o.rows, a->Hq}), "kv_attention: q and o overlap");
-  // the kernels count (unit of 32 tokens, head, 16 rows) in 32 bits, and a launch has fewer than 2^32 threads
-  NEED((unsigned __int128)a->cache.max_pages * 2 * o.Hkv * ((uint64_t)o.rows * (a->Hq / o.Hkv) / 16 + o.B) < (1ull << 32) &&
-           (uint64_t)o.Hkv * ((uint64_t)o.rows * (a->Hq / o.Hkv) / 128 + o.B) < (1ull << 23),
-       "kv_attention: max_pages %u with %u rows of %u heads is too large for one call", a->cache.max_pages, o.rows, a->Hq);
+  o.Hq = a->Hq;
+  NEED(kv_blocks_fit(o) || (kv_runs_fit(o) && !kv_long_rows(o)),
+       "kv_attention: %u rows and %u sequences of %u heads over %u kv heads of max_pages %u are too many for one call", o.rows, o.B, a->Hq,
+       o.Hkv, a->cache.max_pages);
   o.K = (const uint16_t *)((const uint8_t *)a->q_buf + a->q_off);
   o.Ko = (uint16_t *)((uint8_t *)a->o_buf + a->o_off);
-  o.Hq = a->Hq; o.window = a->window; o.sinks = a->sinks;
+  o.window = a->window; o.sinks = a->sinks;
   o.scale = a->scale != 0.0f ? a->scale : 0.08838834764831845f;   // 1 / sqrt(128)
   o.cap = a->cap;
   if (out) *out = o;

@@ -150,6 +150,17 @@ __device__ __forceinline__ f16x8 kv_f16x8(uint32_t a, uint32_t b) {
 }
 #endif
 
+// The kernel over runs of keys counts (unit of 32 tokens, head, 16 rows) in 32 bits, by max_pages, as the lengths are not known
+// here; that over blocks of rows has a workgroup of 512 threads for each block of 256 rows of a kv head, and a launch fewer than
+// 2^32 threads. kv_long_rows: a sequence and kv head have more than a block on average.
+inline bool kv_runs_fit(const KvParams &p) {
+  return (unsigned __int128)p.max_pages * 2 * p.Hkv * ((uint64_t)p.rows * (p.Hq / p.Hkv) / 16 + p.B) < (1ull << 32);
+}
+inline bool kv_blocks_fit(const KvParams &p) {
+  return (uint64_t)p.Hkv * ((uint64_t)p.rows * (p.Hq / p.Hkv) / 256 + p.B) < (1ull << 23);
+}
+inline bool kv_long_rows(const KvParams &p) { return (uint64_t)p.rows * (p.Hq / p.Hkv) > 256ull * p.B; }
+
 // attention over runs of keys: its workspace (partial results of a workgroup's first and last group, and a counter each)
 constexpr uint32_t kva_part(uint32_t rows) { return rows * (KV_D + 2); }          // floats of one partial result
 uint64_t kv_attention_part_bytes(int cus);

@@ -843,9 +843,9 @@ unsigned kv_attention_counters(int cus) { return (unsigned)cus; }
 // Which kernel: blocks of 256 rows where a sequence and kv head have more than that on average and all rows of all heads are
 // more than 20 a CU; runs of keys otherwise. Measured over 2 head layouts, batches of 1 and 8, 1000 and 8000 keys, 16 to 1024
 // rows: 8 heads x 512 rows, 8000 keys: runs 46.5 us, blocks 50.6; x 768: 60.2 and 52.7; 64 heads x 256 rows: 140 and 142 (1000
-// keys: 25.7 and 45.6); x 384: 210 and 157 (37 and 51)
+// keys: 25.7 and 45.6); x 384: 210 and 157 (37 and 51). And where the runs would be too many to count.
 static bool by_blocks(const KvParams &p, int cus) {
-  return (uint64_t)p.rows * (p.Hq / p.Hkv) > 256ull * p.B && (uint64_t)p.rows * p.Hq > 20ull * cus;
+  return (kv_long_rows(p) && (uint64_t)p.rows * p.Hq > 20ull * cus) || !kv_runs_fit(p);
 }
 constexpr uint32_t KVA_BLOCK = 256;               // rows of a block of k_kv_attn_block
 static uint32_t block_items(const KvParams &p) { return (uint32_t)((uint64_t)p.rows * (p.Hq / p.Hkv) / KVA_BLOCK + p.B); }
