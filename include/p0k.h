@@ -178,7 +178,9 @@ typedef struct p0k_batch {
  * still filling is in one, and in the other the one before it, unless a later block took that place before the sequence went
  * back. `held` (optional) says which block each place holds, so that a sequence may go back to any of its tokens (see
  * p0k_kv_append). Buffers: p0k_kv_code_bytes / p0k_kv_scale_bytes / p0k_kv_tail_bytes / p0k_kv_held_bytes; their inner layout
- * is the library's, `held` begins as zeros (as p0k_alloc gives it). Pages of whole blocks may be shared by sequences, as long
+ * is the library's, `held` begins as zeros (as p0k_alloc gives it). A sequence that takes over a slot begins there at token 0,
+ * or with its first tokens in pages that are there already: then the slot's part of `held`, 16 Hkv bytes from 16 Hkv s on, is
+ * set to zeros first. Pages of whole blocks may be shared by sequences, as long
  * as none of them goes back into such a block. A table entry outside [0, pages): the block is not there (not written, not
  * seen, read back as zeros). The page of a block is written when the block becomes whole; until then its entry may stay
  * unset. */
@@ -217,13 +219,12 @@ typedef struct p0k_rope_args {
  * as 0. A block that becomes whole is quantised from the f16 values of all of its tokens: scale = max |x| / 127 in fp32 (1
  * where all are 0), code = x / scale rounded to the nearest, ties to even. So the cache depends on the tokens only, not on
  * how many came with a call. Tokens from max_pages * 64 on are not kept.
- * A sequence may go back (rejected draft tokens): pos may be any place up to its end, but not before the token at which it
- * began in this slot. A call that starts inside a block needs the block's earlier tokens in f16. The tail has them until
- * a token of another block of the same k % 2 is written: always when a sequence goes back no further than to the start of the
- * block before the furthest one that it has written in. Where the tail has them no more, and the cache has `held`, they
- * become what p0k_kv_read gave for them before the call (zeros where the block has no page), and go on from there; without
- * `held` such a call is not allowed, as nothing tells it from others (start it at the block's first token instead: that is
- * right for any block). */
+ * A sequence may go back (rejected draft tokens): pos may be any place up to its end. A call that starts inside a block needs
+ * the block's earlier tokens in f16. The tail has them until a token of another block of the same k % 2 is written: always
+ * when a sequence goes back no further than to the start of the block before the furthest one that it has written in. Where
+ * the tail has them no more, and the cache has `held`, they become what p0k_kv_read gave for them before the call (zeros where
+ * the block has no page), and go on from there; without `held` such a call is not allowed, as nothing tells it from others
+ * (start it at the block's first token instead: that is right for any block). */
 typedef struct p0k_kv_append_args {
   uint32_t struct_size;
   p0k_kv_cache cache;
@@ -232,9 +233,9 @@ typedef struct p0k_kv_append_args {
   const void *v_buf; uint64_t v_off, v_size, v_rs, v_hs;
 } p0k_kv_append_args;
 
-/* kv_read: row r of K and V = the cached token pos[b] + r - cu[b] of sequence b, in f16 (code * scale rounded once; the
- * open block's values as they are), zeros where there is none. len[b] (int32 [B]): tokens that sequence b holds. k and v must not
- * overlap. */
+/* kv_read: row r of K and V = the cached token pos[b] + r - cu[b] of sequence b, in f16 (code * scale in fp32, then rounded
+ * to f16; the open block's values as they are), zeros where there is none. len[b] (int32 [B]): tokens that sequence b holds, or
+ * the first of them, as many as kv_attention may be asked for. k and v must not overlap. */
 typedef struct p0k_kv_read_args {
   uint32_t struct_size;
   p0k_kv_cache cache;
@@ -246,7 +247,10 @@ typedef struct p0k_kv_read_args {
 
 /* kv_attention: O [rows][ldo] f16, head h at column h * 128 = softmax(scale q.k) v over the cached tokens j that the query
  * at token t sees: j <= t and, with a window, j > t - window or j < sinks. The cache holds the batch's own rows already
- * (p0k_kv_append comes first): sequence b has pos[b] + cu[b + 1] - cu[b] tokens. Query head h reads kv head h / (Hq / Hkv).
+ * (p0k_kv_append comes first). Sequence b has pos[b] + cu[b + 1] - cu[b] tokens; it may have more where the cache has `held`
+ * (without it: where the last of these tokens is in a block that the tail holds, or its block's last): queries of a prompt
+ * written at once may come in chunks. The block in which these tokens end is taken in f16 while the tail holds it, from its
+ * codes otherwise. Query head h reads kv head h / (Hq / Hkv).
  * A row that sees nothing is 0 (with offsets that decrease, rows may be left as they are). o and q must not overlap. Zero
  * fields: ldo = Hq * 128, scale = 1 / sqrt(128), window: none, cap: none (cap * tanh(s / cap) otherwise); scale in [2^-40,
  * 2^40], cap in [2^-20, 2^20]. o: 8-byte aligned, ldo a multiple of 4. rows * Hq / 256 + B * Hkv is below 2^23 (or, with at

@@ -363,12 +363,14 @@ __device__ __forceinline__ bool attn_split(const KvParams &p, uint32_t ws, float
       for (int j = 0; j < 8; j++) to[j] = *(const f16x8 *)(t + 512 * j);
     };
     if (NB == 1 && o0 < i1) { open(o0, 0, ko); open(o0, 1, vo); }
+    // (its tokens are in its codes where a later block has taken its place: the call ends before the sequence does)
+    const uint32_t ob = w.end / KV_T;
+    const bool codes = p.held && o0 < i1 && kv_held(p, w.s.slot, hk, 0)[ob & 1] != (int32_t)ob + 1;
 
     // whole blocks, up to 64 units ahead: lane i knows unit c0 + i's page and scales
     constexpr uint32_t NONE = 0xffffffffu;
-    const uint32_t ic = i1 < w.io ? i1 : w.io;
-    for (uint32_t c0 = i0; c0 < ic; c0 += 64) {
-      const uint32_t nc = ic - c0 < 64 ? ic - c0 : 64;
+    for (uint32_t c0 = i0; c0 < i1 && (c0 < w.io || codes); c0 += 64) {
+      uint32_t nc = i1 - c0 < 64 ? i1 - c0 : 64;
       uint32_t pg = NONE;
       float lsk = 1.0f, lsv = 1.0f;
       if (lane < nc) {
@@ -380,6 +382,7 @@ __device__ __forceinline__ bool attn_split(const KvParams &p, uint32_t ws, float
           lsv = sc.y;
         }
       }
+      if (!codes && nc > w.io - c0) nc = w.io - c0;
       // (a unit's keys are asked for when the scores of the one before it are done, its values when that one's are)
       u32x4 kc[4], vc[4];
       auto load = [&](uint32_t i, uint32_t kv, u32x4 *to) {
@@ -400,7 +403,7 @@ __device__ __forceinline__ bool attn_split(const KvParams &p, uint32_t ws, float
       }
     }
     // the open block, in f16
-    for (uint32_t i = o0; i < i1; i++) {
+    for (uint32_t i = codes ? i1 : o0; i < i1; i++) {
       const uint32_t un = unit_of(i);
       if (NB != 1 && i == o0) open(i, 0, ko);
       step(un, 1.0f, 1.0f, false, [&](int tt, int s) { return ko[4 * tt + s]; },
@@ -609,12 +612,16 @@ __global__ __launch_bounds__(64 * NW, 2) void k_kv_attn_block(KvParams p, uint32
   constexpr uint32_t NONE = 0xffffffffu, OPEN = 0xfffffffeu;
   uint32_t pg = NONE;
   float lsk = 1.0f, lsv = 1.0f;
+  // (the open block's tokens are in its codes where a later block has taken its place: the call ends before the sequence does)
+  const uint32_t ob = end / KV_T;
+  const bool tail = !p.held || kv_held(p, s.slot, hk, 0)[ob & 1] == (int32_t)ob + 1;
   auto know = [&](uint32_t c0) {
     pg = NONE;
     lsk = lsv = 1.0f;
     if (c0 + lane < nt) {
       const uint32_t tl = tile_of(c0 + lane);
-      pg = tl == end / KV_T ? OPEN : kv_page(p, s.slot, tl);
+      pg = kv_page(p, s.slot, tl);
+      if (tl == ob && tail) pg = OPEN;
       if (pg < OPEN) {
         const f32x2 sc = *(const f32x2 *)(p.scales + kv_scale_at(p, pg, hk, 0));
         lsk = sc.x;

@@ -209,24 +209,26 @@ __device__ void append_block(const KvParams &p, const KvSeq &s, uint32_t blk, ui
   const uint32_t last = end / KV_T;
   const bool kept = blk + 1 >= last && (blk == k0 || ((blk ^ k0) & 1));
   if (kept) keep(blk, s.pos, end);
-  // lost: the block's tokens before this call's are no longer in the tail in f16; the codes' values take their place
+  // the block's tokens before this call's: in the tail, needed where the block becomes whole
+  const bool whole = (blk + 1) * KV_T <= end;
+  auto before = [&](uint32_t t) { return blk * KV_T + t < s.pos; };
+  if (whole && inside) part.load_tail(p.tail + kv_tail_at(p, s.slot, blk, h, KV), x, sC, before);
+  // or lost, where another block has taken their place there: the codes' values are what is left of them
   const int32_t held0 = (int32_t)__builtin_amdgcn_readlane(places, 0), held1 = (int32_t)__builtin_amdgcn_readlane(places, 1);
-  const bool lost = held && inside && (blk & 1 ? held1 : held0) != (int32_t)blk + 1;
-  if (__builtin_expect(lost, 0)) {
+  if (__builtin_expect(held && inside && (blk & 1 ? held1 : held0) != (int32_t)blk + 1, 0)) {
+    __syncthreads();                             // (all have taken the tail's values from LDS)
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (before(part.tok(i))) x[i] = (u16x8){};
     const uint32_t page = page_of();
-    if (page != 0xffffffffu) {
-      load_codes(p, part, page, h, x, sC, [&](uint32_t t) { return blk * KV_T + t < s.pos; });
-      kv_hold(x);                                // (a page that no call has written)
-    }
+    if (page != 0xffffffffu) load_codes(p, part, page, h, x, sC, before);
+    kv_hold(x);                                  // (a page that no call has written)
     if (kept) keep(blk, 0, s.pos);
   }
-  if ((blk + 1) * KV_T <= end) {
+  if (whole) {
     const uint32_t page = page_of();
     const bool have = page != 0xffffffffu;
-    if (inside && !lost) {
-      part.load_tail(p.tail + kv_tail_at(p, s.slot, blk, h, KV), x, sC, [&](uint32_t t) { return blk * KV_T + t < s.pos; });
-      kv_hold(x);                                // (a tail that no call has written)
-    }
+    if (inside) kv_hold(x);                      // (a tail that no call has written)
     uint32_t mx = kv_amax(x);
     for (int o = 32; o; o >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
     if ((tid & 63) == 0) sMax[tid >> 6] = h_val((uint16_t)mx);
@@ -299,11 +301,21 @@ __device__ void read_block(const KvParams &p, const KvSeq &s, uint32_t blk, uint
   u16x8 x[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) x[i] = (u16x8){};
-  const uint32_t page = blk < len / KV_T ? kv_page(p, s.slot, blk) : 0xffffffffu;
-  if (blk == len / KV_T) {
-    part.load_tail(p.tail + kv_tail_at(p, s.slot, blk, h, KV), x, sC, [&](uint32_t t) { return blk * KV_T + t < len; });
-  } else if (page != 0xffffffffu) {
-    load_codes(p, part, page, h, x, sC, [](uint32_t) { return true; });
+  if (blk < len / KV_T) {
+    const uint32_t page = kv_page(p, s.slot, blk);
+    if (page != 0xffffffffu) load_codes(p, part, page, h, x, sC, [](uint32_t) { return true; });
+  } else if (blk == len / KV_T) {
+    auto there = [&](uint32_t t) { return blk * KV_T + t < len; };
+    const int32_t place = p.held && len % KV_T ? kv_held(p, s.slot, h, KV)[blk & 1] : (int32_t)blk + 1;
+    part.load_tail(p.tail + kv_tail_at(p, s.slot, blk, h, KV), x, sC, there);
+    if (__builtin_expect(place != (int32_t)blk + 1, 0)) {
+      // a later block has taken its place, as the sequence has more tokens than the call asks for: they are in its codes
+      __syncthreads();                            // (all have taken the tail's values from LDS)
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[i] = (u16x8){};
+      const uint32_t page = kv_page(p, s.slot, blk);
+      if (page != 0xffffffffu) load_codes(p, part, page, h, x, sC, there);
+    }
   }
   uint16_t *Y = (KV ? p.Vo : p.Ko) + (KV ? p.vhs : p.khs) * h;
 #pragma unroll
