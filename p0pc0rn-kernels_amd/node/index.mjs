@@ -294,11 +294,16 @@ function rope(gpu, a) {
 /** kvCache(gpu, {Hkv, pages, slots, maxPages, table}): the buffers of a cache, `pages` pages of 64 tokens for `slots` sequences of
  *  up to maxPages blocks. table: Int32 [slots][maxPages] buffer of page numbers (default: sequence s owns pages s * maxPages on) */
 function kvCache(gpu, o) {
-  const [code, scale, tail, held] = call(addon().kvBytes, o.pages, o.slots, o.Hkv);
-  let table = o.table;
-  if (!table) table = gpu.upload(Int32Array.from({ length: o.slots * o.maxPages }, (_, i) => (i < o.pages ? i : -1)), 'kv table');
-  return { code: gpu.buffer(code, 'kv codes'), scale: gpu.buffer(scale, 'kv scales'), tail: gpu.buffer(tail, 'kv tail'),
-    held: gpu.buffer(held, 'kv held'), table, pages: o.pages, slots: o.slots, maxPages: o.maxPages, Hkv: o.Hkv };
+  const sizes = call(addon().kvBytes, o.pages, o.slots, o.Hkv), made = [];
+  const keep = (b) => { made.push(b); return b; };
+  try {
+    const table = o.table || keep(gpu.upload(Int32Array.from({ length: o.slots * o.maxPages }, (_, i) => (i < o.pages ? i : -1)), 'kv table'));
+    const [code, scale, tail, held] = ['codes', 'scales', 'tail', 'held'].map((n, i) => keep(gpu.buffer(sizes[i], 'kv ' + n)));
+    return { code, scale, tail, held, table, pages: o.pages, slots: o.slots, maxPages: o.maxPages, Hkv: o.Hkv };
+  } catch (e) {
+    made.forEach((b) => gpu.free(b));
+    throw e;
+  }
 }
 
 /** kvAppend(gpu, {cache, batch, k, v}): rows of K / V into the cache */

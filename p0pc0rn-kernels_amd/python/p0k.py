@@ -566,19 +566,24 @@ class Device:
         64 tokens for all kv heads, `slots` sequences of up to max_pages blocks. table: int32 [slots][max_pages] page
         numbers, -1 where there is none; without one, sequence s owns pages s * max_pages on. `held` lets sequences go
         back to any of their tokens."""
-        L, own = lib(), table is None
-        if own:
-            t = np.full((slots, max_pages), -1, np.int32)
-            n = min(pages, slots * max_pages)
-            t.reshape(-1)[:n] = np.arange(n)
-            table = self.upload(t)
-        return {"code": self.buffer(L.p0k_kv_code_bytes(pages, Hkv)), "scale": self.buffer(L.p0k_kv_scale_bytes(pages, Hkv)),
-                "tail": self.buffer(L.p0k_kv_tail_bytes(slots, Hkv)), "held": self.buffer(L.p0k_kv_held_bytes(slots, Hkv)), "table": table,
-                "pages": pages, "slots": slots, "max_pages": max_pages, "Hkv": Hkv, "own_table": own}
+        L, cache = lib(), {"table": table, "own_table": table is None}
+        try:
+            if table is None:
+                t = np.full((slots, max_pages), -1, np.int32)
+                n = min(pages, slots * max_pages)
+                t.reshape(-1)[:n] = np.arange(n)
+                cache["table"] = self.upload(t)
+            for name, size in (("code", L.p0k_kv_code_bytes(pages, Hkv)), ("scale", L.p0k_kv_scale_bytes(pages, Hkv)),
+                               ("tail", L.p0k_kv_tail_bytes(slots, Hkv)), ("held", L.p0k_kv_held_bytes(slots, Hkv))):
+                cache[name] = self.buffer(size)
+        except Exception:
+            self.kv_cache_free(cache)
+            raise
+        return {**cache, "pages": pages, "slots": slots, "max_pages": max_pages, "Hkv": Hkv}
 
     def kv_cache_free(self, cache):
         """gives the cache's buffers back (a table that came from the caller stays the caller's)"""
-        for n in ("code", "scale", "tail", "held") + (("table",) if cache["own_table"] else ()):
+        for n in ("code", "scale", "tail", "held") + (("table",) if cache.get("own_table") else ()):
             self.free(cache.get(n))
 
     def kv_append_raw(self, s):
