@@ -265,6 +265,9 @@ const operand = (d, name, x) => {
     [name + '_rs']: x.rs || 0, [name + '_hs']: x.hs || 0 });
 };
 function batchDesc(d, b) {
+  // (left out, they would be 0: a call that does nothing)
+  if (!(b.rows >= 0)) throw new Error(`batch: rows is ${b.rows}`);
+  if (b.cu && !(b.B >= 0)) throw new Error(`batch: B is ${b.B}`);
   for (const n of ['pos', 'cu', 'slot']) operand(d, n, b[n]);
   d.B = b.B || 0; d.rows = b.rows;
 }
@@ -281,6 +284,7 @@ const ROPE_MODE = { __proto__: null, interleaved: 0, half: 1 }, ROPE_SCALING = {
 function rope(gpu, a) {
   const sc = a.scaling || { kind: 'plain' };
   const mode = ROPE_MODE[a.mode || 'interleaved'], scaling = ROPE_SCALING[sc.kind];
+  if (!(a.H >= 0)) throw new Error(`rope: H is ${a.H}`);
   if (mode === undefined) throw new Error(`rope: unknown mode ${a.mode}`);
   if (scaling === undefined) throw new Error(`rope: unknown scaling kind ${sc.kind}`);
   const d = { H: a.H, rd: a.rd || 0, mode, scaling, theta: a.theta || 0,

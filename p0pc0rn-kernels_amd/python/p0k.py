@@ -173,7 +173,7 @@ def _set_batch(s, b, resolve):
     for n in ("pos", "cu", "slot"):
         if b.get(n) is not None:
             _set_operand(s, n, b[n], resolve)
-    s.B, s.rows = _get(b, "B", 0), b["rows"]
+    s.B, s.rows = b["B"] if b.get("cu") is not None else 0, b["rows"]
 
 
 def _set_cache(s, c, resolve):

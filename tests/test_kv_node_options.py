@@ -35,3 +35,28 @@ def test_rope_options_of_the_python_binding(o):
     x = np.zeros(128, np.float16)
     with pytest.raises(KeyError):
         p0k.rope_args({"x": x, "H": 1, "batch": {"pos": np.zeros(1, np.int32), "rows": 1}, **o}, p0k.numpy_resolve)
+
+
+NEEDED = [("rope", {"H": None}, "rope: H is"), ("rope", {"batch": {"rows": None}}, "batch: rows is"), ("rope", {"batch": {"B": None}}, "batch: B is"),
+          ("kvAppend", {"batch": {"rows": None}}, "batch: rows is"), ("kvRead", {"batch": {"B": None}}, "batch: B is"),
+          ("kvAttention", {"batch": {"rows": "many"}}, "batch: rows is many"), ("kvAttention", {}, "NULL context")]
+
+
+def test_numbers_that_are_left_out():
+    """rows, sequences and heads that are not given are not taken as none"""
+    src = ("import('%s/p0pc0rn-kernels_amd/node/index.mjs').then((m) => console.log(JSON.stringify(%s.map(([f, o]) => {"
+           "const u = (x) => Object.fromEntries(Object.entries(x).map(([k, v]) => [k, v === null ? undefined : v]));"
+           "const b = { ptr: 16n, size: 4096 }, batch = { pos: b, cu: b, B: 1, rows: 1, ...u(o.batch || {}) };"
+           "try { m[f]({ ctx: null }, { cache: {}, x: b, k: b, v: b, q: b, o: b, len: b, Hq: 1, H: 1, ...u(o), batch }); return null; }"
+           " catch (e) { return e.message; } }))))" % (ROOT, json.dumps([c[:2] for c in NEEDED])))
+    r = subprocess.run([NODE, "-e", src], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stderr
+    for c, got in zip(NEEDED, json.loads(r.stdout)):
+        assert got and c[2] in got, (c, got)
+
+
+def test_numbers_that_are_left_out_of_the_python_binding():
+    x, i = np.zeros(128, np.float16), np.zeros(2, np.int32)
+    for a in ({"H": 1, "batch": {"pos": i, "cu": i, "rows": 1}}, {"H": 1, "batch": {"pos": i, "cu": i, "B": 1}}, {"batch": {"pos": i, "rows": 1}}):
+        with pytest.raises(KeyError):
+            p0k.rope_args({"x": x, **a}, p0k.numpy_resolve)
