@@ -92,8 +92,8 @@ __device__ __forceinline__ float rlf(float v, uint32_t l) { return __uint_as_flo
 // in f16; the scales stay in fp32: the keys' multiplies the scores, and O is held in units of the current block's value scale.
 // P is rounded to f16 (the products have no wider operand at this rate); sums, maxima and O are fp32.
 //
-// HBM-bound: 48 sequences of 900 to 6000 tokens, 8 kv heads (349 MB) 63 us, of which the keys' stream takes 50 (7 TB/s); one
-// sequence of 3777 tokens (7.8 MB) 9.8 us: about 2 us until the first codes are asked for, 1.4 for a unit, 6 for the exchanges.
+// HBM-bound: 48 sequences of 900 to 6000 tokens, 8 kv heads (349 MB) 64 us, of which the keys' stream takes 50 (7 TB/s); one
+// sequence of 3777 tokens (7.8 MB) 9.9 us: about 2 us until the first codes are asked for, 1.4 for a unit, 6 for the exchanges.
 // NB: blocks of 16 or 32 rows. 16 read the keys of 17 and more rows twice and more, but start and end sooner; the result is
 // false (and nothing done) where 32 are the better choice, see k_kv_attn_split.
 constexpr int KVA_NW = 8;                         // waves of a workgroup
@@ -554,7 +554,7 @@ __global__ __launch_bounds__(64 * KVA_NW, 2) void k_kv_attn_split(KvParams p, ui
 // V^T P as 32x32x16 products, a lane owning a row. The cache's order of tokens is that of the score registers, so V^T needs no
 // transposing read. The keys' scale multiplies the scores. The values' scale goes into the exponent: O is held in units of
 // `ref`, which moves (and O with it) only when a block's scale leaves [ref, 64 ref] (P is at most 2^8 * 64 then, inside f16).
-// 5003 queries of 32 heads over their own 5003 tokens: 241 us, 0.85 PFLOP/s; VALU and MFMA share the time (8 VALU per MFMA).
+// 5003 queries of 32 heads over their own 5003 tokens: 245 us, 0.84 PFLOP/s; VALU and MFMA share the time (8 VALU per MFMA).
 template <int NW, bool CAP>
 __global__ __launch_bounds__(64 * NW, 2) void k_kv_attn_block(KvParams p, uint32_t items, uint32_t S, float *part) {
   constexpr uint32_t RB = 32 * NW, NP = 512 / (64 * NW);                          // pieces of 16 codes a thread moves, keys and values each

@@ -75,8 +75,9 @@ __device__ __forceinline__ void kv_hold(u16x8 *x) {       // infinities to the l
 // registers from the first load to the last store. Keys: token tid / 4, d 16 c .. + 15 and 64 + 16 c .. (c = tid % 4): whole
 // pieces of the cache. Values: tokens 4 (tid / 16) .. + 3, d 8 (tid % 16) .. + 7: the four tokens of a d are a word of a
 // piece, and pieces are put together in LDS.
-// 5000 rows of 8 heads: append 14.3 us (31 MB, 2.2 TB/s: the loads of all workgroups, then 5.5 us of VALU), read 8.8; 16384
-// rows read back 23.8 us (100 MB, 4.2 TB/s).
+// 5000 rows of 8 heads: append 12.9 us (31 MB, 2.4 TB/s: the loads of all workgroups, then 5.5 us of VALU), read 9.0; 16384
+// rows read back 23.0 us (100 MB, 4.4 TB/s). One token of 64 sequences: append 5.7 us (5.0 without `held`, whose entries come from
+// memory with the rows).
 template <int KV>
 struct Part {
   uint32_t tid;
