@@ -179,11 +179,11 @@ typedef struct p0k_batch {
  * back. `held` (optional) says which block each place holds, so that a sequence may go back to any of its tokens (see
  * p0k_kv_append). Buffers: p0k_kv_code_bytes / p0k_kv_scale_bytes / p0k_kv_tail_bytes / p0k_kv_held_bytes; their inner layout
  * is the library's, `held` begins as zeros (as p0k_alloc gives it). A sequence that takes over a slot begins there at token 0,
- * or with its first tokens in pages that are there already: then the slot's part of `held`, 16 Hkv bytes from 16 Hkv s on, is
- * set to zeros first. Pages of whole blocks may be shared by sequences, as long
- * as none of them goes back into such a block. A table entry outside [0, pages): the block is not there (not written, not
- * seen, read back as zeros). The page of a block is written when the block becomes whole; until then its entry may stay
- * unset. */
+ * or with its first tokens in pages that are there already: then the slot's part of `held`, p0k_kv_held_bytes(1, Hkv) from s
+ * times that on, is set to zeros first. To continue a sequence in another slot as well, copy its parts of both `tail` and
+ * `held` there. Pages of whole blocks may be shared by sequences, as long as none of them goes back into such a block. A table
+ * entry outside [0, pages): the block is not there (not written, not seen, read back as zeros). The page of a block is written
+ * when the block becomes whole; until then its entry may stay unset. */
 typedef struct p0k_kv_cache {
   void *code_buf; uint64_t code_off, code_size;           /* codes, tail: 16-byte aligned; scales: 8-byte */
   float *scale_buf; uint64_t scale_off, scale_size;

@@ -112,3 +112,24 @@ def test_slot_taken_over(cache):  # noqa: F811
     c.check_all()
     attend(c, "runs16", [(0, 357, 1), (0, 157, 1), (0, 100, 5), (1, 699, 1)], 8, rng)
     assert c.ref.lost == 0
+
+
+@pytest.mark.gpu
+def test_sequence_copied_to_another_slot(cache):  # noqa: F811
+    """a sequence goes on in two slots that share its whole pages: the second has a copy of the first one's parts of tail and held"""
+    rng = np.random.default_rng(115)
+    c = cache(2, 3, 12)
+    c.ref = Part(3, 2)
+    c.append([(0, 0, 500), (1, 0, 205), (2, 0, 400)], rng)
+    for n, size in (("tail", 2 * 65536), ("held", 32)):
+        c.dev.copy(c.c[n], 2 * size, c.c[n], size, size)
+    c.table[2, :3] = c.table[1, :3]
+    c.dev.upload(c.table, c.tb)
+    for x in (c.ref.k, c.ref.v, c.ref.tail):
+        x[2] = x[1][:] if isinstance(x[1], list) else x[1]
+    c.check_all()
+    c.append([(2, 205, 7), (1, 205, 3)], rng)
+    c.append([(1, 208, 100), (2, 200, 90), (0, 500, 1)], rng)        # (the copy goes back in its own block)
+    c.check_all()
+    attend(c, "runs16", [(1, 300, 8), (2, 289, 1), (0, 499, 2), (2, 140, 3)], 8, rng)
+    assert c.ref.lost == 0
